@@ -229,6 +229,89 @@ mr_status mr_mxfp4_gather_mm_f32(mr_ctx* ctx, const float* x, int64_t tokens,
 mr_status mr_mxfp4_dequantize(mr_ctx* ctx, const mr_mxfp4_desc* w, float* out,
                               void* stream);
 
+/* Quantisation to MXFP4 (OCP MX): per block of 32 elements the exponent is
+ * floor(log2 max|x|) - 2, clamped to e8m0, and each element the nearest e2m1
+ * number of x * 2^-exponent, ties to the even code, saturating at 6. A block
+ * with an infinity or NaN gets exponent 255 (reads back as NaN) and zero
+ * codes. x: bf16, f16 or f32 rows of in_features (a multiple of 32) elements,
+ * x_stride elements apart; packed [rows, in/8] and scales [rows, in/32] as in
+ * mr_mxfp4_desc (an expert stack is experts * out rows). values (may be NULL,
+ * 16-byte aligned): [rows, in] of x's type, the numbers the codes stand for,
+ * rounded to that type. rows may be 0. Up to 2^35 elements a call. */
+mr_status mr_mxfp4_quantize(mr_ctx* ctx, const void* x, mr_dtype dtype, int64_t rows,
+                            int64_t in_features, int64_t x_stride, uint32_t* packed,
+                            uint8_t* scales, void* values, void* stream);
+/* The same of h = silu(gate) * up (fp32), for gate_up rows [gate | up] of
+ * 2 * inter elements, stride elements apart: what the second expert product
+ * takes, without h in memory. swiglu_limit > 0: gate <= L, -L <= up <= L. */
+mr_status mr_mxfp4_quantize_swiglu(mr_ctx* ctx, const void* gate_up, mr_dtype dtype, int64_t rows,
+                                   int64_t inter, int64_t stride, float swiglu_limit,
+                                   uint32_t* packed, uint8_t* scales, void* stream);
+
+/* ------------------------------------------------- tokens sorted by expert
+ * The pairs (token t, slot j) of a router's choice, pair p = t * top_k + j,
+ * in the order of their experts (pairs of one expert keep their order), and
+ * the rows of the tokens moved there and back. No counterpart in the
+ * reference, whose gather takes ids (AffineWeights.swift:283-318): this is
+ * for experts that work on contiguous rows, and for training them. */
+typedef struct mr_sorted {
+  const int32_t* order;   /* [tokens * top_k] the pair at each sorted row; -1 in the
+                             rows past offsets[experts]                          */
+  const int32_t* inverse; /* [tokens, top_k] the row of each pair, -1: no expert  */
+  const int32_t* offsets; /* [experts + 1] first row of each expert               */
+  int64_t tokens;         /* may be 0                                             */
+  int32_t top_k;          /* <= 1024; tokens * top_k < 2^31                       */
+  int32_t experts;        /* <= 1024                                              */
+} mr_sorted;
+
+/* ids int32 [tokens, top_k] -> order, inverse, offsets (device buffers). An id
+ * of -1 is a slot without an expert (one held by another rank, a dropped
+ * token); any other id outside [0, experts) is treated so too and sets
+ * MR_DEVERR_BAD_EXPERT_ID. Deterministic. */
+mr_status mr_moe_sort(mr_ctx* ctx, const int32_t* ids, int64_t tokens, int32_t top_k,
+                      int32_t experts, int32_t* order, int32_t* inverse, int32_t* offsets,
+                      void* stream);
+/* xs[r] = x[order[r] / top_k]; rows without a pair are zero. x: rows of
+ * `hidden` bf16, f16 or f32 elements, x_stride elements apart; xs contiguous
+ * [tokens * top_k, hidden]. */
+mr_status mr_moe_dispatch(mr_ctx* ctx, const void* x, mr_dtype dtype, int64_t x_stride,
+                          int64_t hidden, const mr_sorted* plan, void* xs, void* stream);
+/* Its gradient: dx[t] = sum_j dxs[inverse[t, j]], fp32 sums in slot order. */
+mr_status mr_moe_dispatch_backward(mr_ctx* ctx, const void* dxs, mr_dtype dtype,
+                                   int64_t dxs_stride, int64_t hidden, const mr_sorted* plan,
+                                   void* dx, void* stream);
+/* out[t] = base[t] + sum_j weights[t, j] * ys[inverse[t, j]] in fp32 and slot
+ * order; weights fp32 [tokens, top_k]; base (the shared expert's rows) and out
+ * contiguous [tokens, hidden] of ys's type, base may be NULL or out itself. A
+ * slot without an expert adds nothing, whatever its weight. */
+mr_status mr_moe_combine(mr_ctx* ctx, const void* ys, mr_dtype dtype, int64_t ys_stride,
+                         int64_t hidden, const float* weights, const void* base,
+                         const mr_sorted* plan, void* out, void* stream);
+/* Its gradients: dys[r] = weights(pair) * dout[t] (zero in rows without a
+ * pair; the type of ys), dweights[t, j] = <dout[t], ys[inverse[t, j]]> in fp32
+ * (zero for a slot without an expert). The gradient of base is dout itself. */
+mr_status mr_moe_combine_backward(mr_ctx* ctx, const void* dout, int64_t dout_stride,
+                                  const void* ys, int64_t ys_stride, mr_dtype dtype,
+                                  int64_t hidden, const float* weights, const mr_sorted* plan,
+                                  void* dys, float* dweights, void* stream);
+
+/* --------------------------------------- MXFP4 x MXFP4 products (4 bits in)
+ * Both operands MXFP4, on the tensor cores' block-scaled 4-bit form: every
+ * e2m1 product and its two scales are exact, sums are fp32. Any valid width
+ * (in % 32 == 0); packed 16-byte aligned. out bf16 or f32, contiguous. */
+
+/* out[r, o] = a[r] . w[o] for single matrices a [rows, in] (its `out_features`
+ * are the rows; they may be 0) and w [out, in]. */
+mr_status mr_mxfp4_scaled_mm(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
+                             mr_dtype out_dtype, void* out, void* stream);
+/* Over sorted rows: out[r] = w[e] . a[r] for offsets[e] <= r < offsets[e + 1],
+ * zeros in the rows past offsets[experts]; out [tokens * top_k, out]. a holds
+ * the sorted rows [tokens * top_k, in], or with by_token the tokens' rows
+ * [tokens, in]: row r then takes a[order[r] / top_k], read in place. */
+mr_status mr_mxfp4_grouped_mm(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
+                              const mr_sorted* plan, int by_token, mr_dtype out_dtype, void* out,
+                              void* stream);
+
 /* ---------------------------------------------------------------- router
  * K3Router.select (Sources/ModelAdapters/Operators/MoE.swift:77-150),
  * DeepSeekV4Router.select (Operators/DeepSeekV4Routing.swift:100-280),

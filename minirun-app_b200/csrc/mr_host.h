@@ -1,0 +1,35 @@
+// mr_host.h — what the host sides of the entry points share.
+#pragma once
+
+#include "mr_common.cuh"
+
+#include <new>
+
+namespace mr {
+
+// No C++ exception leaves the C ABI: what building a message may throw is an
+// allocation failure.
+template <typename F>
+inline mr_status guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return MR_ERR_OUT_OF_MEMORY;
+  } catch (...) {
+    return MR_ERR_INVALID_ARGUMENT;
+  }
+}
+
+// The context's device, for callers whose current device is another one.
+inline cudaError_t set_device(const mr_ctx* ctx) {
+  int cur = -1;
+  const cudaError_t e = cudaGetDevice(&cur);
+  return e == cudaSuccess && cur != ctx->device ? cudaSetDevice(ctx->device) : e;
+}
+
+// The shape and pointers of sorted tokens (mr_sort.cu).
+mr_status check_plan(mr_ctx* ctx, const mr_sorted* s);
+
+inline uint64_t addr(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+}  // namespace mr

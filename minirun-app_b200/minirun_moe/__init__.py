@@ -15,6 +15,10 @@ from .moe import (MoELayer, ResidentExpertBackend, RouterConfig, TokenExpertMap,
 from .checkpoint import Checkpoint, SafetensorsError, SafetensorsFile, write_safetensors
 from .mxfp4 import (MXFP4BridgeError, MXFP4Weights, mxfp4_dequantize, mxfp4_gather_mm,
                     mxfp4_gather_mm_f32, mxfp4_mm, mxfp4_mm_f32, mxfp4_validate)
+from .mxfp4_scaled import (mxfp4_grouped_mm, mxfp4_quantize, mxfp4_quantize_swiglu,
+                           mxfp4_scaled_mm)
+from .sorted_tokens import (SortedTokens, moe_combine, moe_combine_backward, moe_dispatch,
+                            moe_dispatch_backward, moe_sort)
 from .k3 import K3MoE, K3Projection, dense_mm_f32, situ
 from .tiles import (ExpertContainers, TileContainer, TileContainerError, write_container,
                     write_expert_containers)
@@ -29,4 +33,7 @@ __all__ = [
     "write_safetensors", "TokenExpertMap", "router_select_hashed", "MXFP4BridgeError",
     "MXFP4Weights", "mxfp4_dequantize", "mxfp4_gather_mm", "mxfp4_mm", "mxfp4_validate",
     "mxfp4_gather_mm_f32", "mxfp4_mm_f32", "K3MoE", "K3Projection", "dense_mm_f32", "situ",
+    "mxfp4_quantize", "mxfp4_quantize_swiglu", "mxfp4_scaled_mm", "mxfp4_grouped_mm",
+    "SortedTokens", "moe_sort", "moe_dispatch", "moe_dispatch_backward", "moe_combine",
+    "moe_combine_backward",
 ]

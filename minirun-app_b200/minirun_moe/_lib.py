@@ -48,6 +48,11 @@ class mr_mxfp4_desc(C.Structure):
                 ("out_features", C.c_int64), ("in_features", C.c_int64)]
 
 
+class mr_sorted(C.Structure):
+    _fields_ = [("order", vp), ("inverse", vp), ("offsets", vp), ("tokens", C.c_int64),
+                ("top_k", C.c_int32), ("experts", C.c_int32)]
+
+
 class mr_router_config(C.Structure):
     _fields_ = [("experts", C.c_int32), ("top_k", C.c_int32), ("scoring", C.c_int),
                 ("renorm", C.c_int), ("renorm_eps", C.c_float), ("routed_scale", C.c_float),
@@ -143,6 +148,23 @@ SIGNATURES = {
     "mr_mxfp4_mm_f32": (C.c_int, [vp, vp, C.c_int64, C.POINTER(mr_mxfp4_desc), vp, vp]),
     "mr_mxfp4_gather_mm_f32": (C.c_int, [vp, vp, C.c_int64, vp, C.c_int32,
                                          C.POINTER(mr_mxfp4_desc), vp, vp]),
+    "mr_mxfp4_quantize": (C.c_int, [vp, vp, C.c_int, C.c_int64, C.c_int64, C.c_int64, vp, vp, vp,
+                                    vp]),
+    "mr_mxfp4_quantize_swiglu": (C.c_int, [vp, vp, C.c_int, C.c_int64, C.c_int64, C.c_int64,
+                                           C.c_float, vp, vp, vp]),
+    "mr_mxfp4_scaled_mm": (C.c_int, [vp, C.POINTER(mr_mxfp4_desc), C.POINTER(mr_mxfp4_desc),
+                                     C.c_int, vp, vp]),
+    "mr_mxfp4_grouped_mm": (C.c_int, [vp, C.POINTER(mr_mxfp4_desc), C.POINTER(mr_mxfp4_desc),
+                                      C.POINTER(mr_sorted), C.c_int, C.c_int, vp, vp]),
+    "mr_moe_sort": (C.c_int, [vp, vp, C.c_int64, C.c_int32, C.c_int32, vp, vp, vp, vp]),
+    "mr_moe_dispatch": (C.c_int, [vp, vp, C.c_int, C.c_int64, C.c_int64, C.POINTER(mr_sorted),
+                                  vp, vp]),
+    "mr_moe_dispatch_backward": (C.c_int, [vp, vp, C.c_int, C.c_int64, C.c_int64,
+                                           C.POINTER(mr_sorted), vp, vp]),
+    "mr_moe_combine": (C.c_int, [vp, vp, C.c_int, C.c_int64, C.c_int64, vp, vp,
+                                 C.POINTER(mr_sorted), vp, vp]),
+    "mr_moe_combine_backward": (C.c_int, [vp, vp, C.c_int64, vp, C.c_int64, C.c_int, C.c_int64,
+                                          vp, C.POINTER(mr_sorted), vp, vp, vp]),
     "mr_dense_mm_f32": (C.c_int, [vp, vp, C.c_int64, vp, C.c_int, C.c_int64, C.c_int64, vp, vp]),
     "mr_k3_situ": (C.c_int, [vp, vp, C.c_int64, C.c_int64, C.c_float, C.c_float, vp, vp]),
     "mr_k3_moe_validate": (C.c_int, [C.POINTER(mr_k3_moe), C.c_char_p, C.c_size_t]),

@@ -112,6 +112,11 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _raw_stream(device: torch.device) -> int:
+    """The current stream of a tensor's device."""
+    return torch.cuda.current_stream(device).cuda_stream
+
+
 def _ptr(t: torch.Tensor | None) -> C.c_void_p:
     return C.c_void_p(0 if t is None else t.data_ptr())
 

@@ -1,0 +1,217 @@
+"""Tokens sorted by expert and back, over libminirun_moe's C ABI.
+
+A router chooses ``top_k`` experts a token (``Selection.ids``). ``moe_sort``
+orders the (token, slot) pairs by expert, ``moe_dispatch`` copies the tokens'
+rows into that order, the experts work on contiguous rows, and
+``moe_combine`` brings their rows back, weighted and summed. Both copies have
+their gradients, as functions and through torch's autograd: where an input
+requires a gradient, ``moe_dispatch`` and ``moe_combine`` record it.
+
+An id of -1 is a slot without an expert: it takes no expert's row, its sorted
+row comes after all experts' and holds zeros, and the combine adds nothing.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+from .bridge import AffineBridgeError, Context, _raw_stream
+
+_ROW_DTYPES = {torch.bfloat16: L.MR_DTYPE_BF16, torch.float16: L.MR_DTYPE_F16,
+               torch.float32: L.MR_DTYPE_F32}
+
+
+class SortedTokens:
+    """What ``moe_sort`` returns: ``order`` [tokens * top_k] (the pair
+    ``token * top_k + slot`` at each sorted row, -1 past the last expert's),
+    ``inverse`` [tokens, top_k] (the row of each pair, -1 without an expert)
+    and ``offsets`` [experts + 1] (first row of each expert), int32."""
+
+    def __init__(self, order: torch.Tensor, inverse: torch.Tensor, offsets: torch.Tensor,
+                 experts: int):
+        if inverse.dim() != 2 or order.shape != (inverse.numel(),):
+            raise AffineBridgeError(
+                f"inverse must be [tokens, top_k] and order [tokens * top_k], got "
+                f"{list(inverse.shape)} and {list(order.shape)}")
+        if offsets.shape != (experts + 1,):
+            raise AffineBridgeError(
+                f"offsets must be [{experts + 1}] for {experts} experts, got "
+                f"{list(offsets.shape)}")
+        for t in (order, inverse, offsets):
+            if t.dtype != torch.int32 or not t.is_contiguous() or not t.is_cuda:
+                raise AffineBridgeError("sorted tokens are contiguous CUDA int32 tensors")
+            if t.device != order.device:
+                raise AffineBridgeError("sorted tokens must be on one device")
+        self._fill(order, inverse, offsets, experts)
+
+    def _fill(self, order, inverse, offsets, experts):
+        self.order, self.inverse, self.offsets = order, inverse, offsets
+        self.experts = experts
+        self.tokens, self.top_k = inverse.shape
+        self.device = order.device
+        self._c = L.mr_sorted(order.data_ptr(), inverse.data_ptr(), offsets.data_ptr(),
+                              self.tokens, self.top_k, experts)
+        self._ref = C.byref(self._c)
+
+    @property
+    def rows(self) -> int:
+        return self.tokens * self.top_k
+
+
+def moe_sort(ids: torch.Tensor, experts: int) -> SortedTokens:
+    """The pairs of ``ids`` [tokens, top_k] in the order of their experts, stable."""
+    if ids.dim() != 2 or not ids.is_cuda:
+        raise AffineBridgeError("ids must be a CUDA [tokens, top_k] tensor")
+    if ids.dtype != torch.int32:
+        if ids.dtype != torch.int64:
+            raise AffineBridgeError(f"ids must be int32 or int64, got {ids.dtype}")
+        ids = ids.to(torch.int32)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    T, k = ids.shape
+    dev = ids.device
+    P = T * k
+    # one allocation: inverse, order, offsets
+    mem = torch.empty((2 * P + max(experts, 0) + 1,), dtype=torch.int32, device=dev)
+    order, inverse, offsets = mem[:P], mem[P:2 * P].view(T, k), mem[2 * P:]
+    ctx = Context.get(dev.index)
+    at = mem.data_ptr()
+    ctx.check("mr_moe_sort", L.load().mr_moe_sort(
+        ctx.handle, ids.data_ptr(), T, k, experts, at, at + 4 * P, at + 8 * P,
+        _raw_stream(dev)))
+    s = SortedTokens.__new__(SortedTokens)
+    s._fill(order, inverse, offsets, experts)
+    return s
+
+
+def _rows(name: str, t: torch.Tensor, rows: int, plan: SortedTokens) -> torch.Tensor:
+    """[rows, hidden] with contiguous rows, of a supported type, on the plan's device."""
+    if t.dim() != 2 or t.shape[0] != rows:
+        raise AffineBridgeError(f"{name} must be [{rows}, hidden], got {list(t.shape)}")
+    if t.dtype not in _ROW_DTYPES:
+        raise AffineBridgeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if t.device != plan.device:
+        raise AffineBridgeError(f"{name} is on {t.device}, the sorted tokens on {plan.device}")
+    if t.stride(1) != 1 or (rows > 1 and t.stride(0) < t.shape[1]):
+        return t.contiguous()
+    return t
+
+
+def _stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def _weights(w: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
+    if w.shape != plan.inverse.shape or w.dtype != torch.float32 or w.device != plan.device:
+        raise AffineBridgeError(
+            f"weights must be [{plan.tokens}, {plan.top_k}] float32 on {plan.device}, got "
+            f"{list(w.shape)} {w.dtype} on {w.device}")
+    return w if w.is_contiguous() else w.contiguous()
+
+
+def _dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
+    x = _rows("x", x, plan.tokens, plan)
+    H = x.shape[1]
+    xs = torch.empty((plan.rows, H), dtype=x.dtype, device=x.device)
+    ctx = Context.get(x.device.index)
+    ctx.check("mr_moe_dispatch", L.load().mr_moe_dispatch(
+        ctx.handle, x.data_ptr(), _ROW_DTYPES[x.dtype], _stride(x), H, plan._ref,
+        xs.data_ptr(), _raw_stream(x.device)))
+    return xs
+
+
+def moe_dispatch_backward(dxs: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
+    """Gradient of ``moe_dispatch``: ``dx[t] = sum_j dxs[inverse[t, j]]``, fp32 sums."""
+    dxs = _rows("dxs", dxs, plan.rows, plan)
+    H = dxs.shape[1]
+    dx = torch.empty((plan.tokens, H), dtype=dxs.dtype, device=dxs.device)
+    ctx = Context.get(dxs.device.index)
+    ctx.check("mr_moe_dispatch_backward", L.load().mr_moe_dispatch_backward(
+        ctx.handle, dxs.data_ptr(), _ROW_DTYPES[dxs.dtype], _stride(dxs), H, plan._ref,
+        dx.data_ptr(), _raw_stream(dxs.device)))
+    return dx
+
+
+def _combine(ys, weights, plan, base) -> torch.Tensor:
+    ys = _rows("ys", ys, plan.rows, plan)
+    H = ys.shape[1]
+    weights = _weights(weights, plan)
+    if base is not None:
+        if base.shape != (plan.tokens, H) or base.dtype != ys.dtype or base.device != ys.device:
+            raise AffineBridgeError(
+                f"base must be [{plan.tokens}, {H}] {ys.dtype} on {ys.device}, got "
+                f"{list(base.shape)} {base.dtype} on {base.device}")
+        base = base.contiguous()
+    out = torch.empty((plan.tokens, H), dtype=ys.dtype, device=ys.device)
+    ctx = Context.get(ys.device.index)
+    ctx.check("mr_moe_combine", L.load().mr_moe_combine(
+        ctx.handle, ys.data_ptr(), _ROW_DTYPES[ys.dtype], _stride(ys), H, weights.data_ptr(),
+        None if base is None else base.data_ptr(), plan._ref, out.data_ptr(),
+        _raw_stream(ys.device)))
+    return out
+
+
+def moe_combine_backward(dout: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor,
+                         plan: SortedTokens) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gradients ``(dys, dweights)`` of ``moe_combine``; that of ``base`` is ``dout``."""
+    ys = _rows("ys", ys, plan.rows, plan)
+    dout = _rows("dout", dout, plan.tokens, plan)
+    H = ys.shape[1]
+    if dout.dtype != ys.dtype or dout.shape[1] != H:
+        raise AffineBridgeError(
+            f"dout must be [{plan.tokens}, {H}] {ys.dtype}, got {list(dout.shape)} {dout.dtype}")
+    weights = _weights(weights, plan)
+    dys = torch.empty((plan.rows, H), dtype=ys.dtype, device=ys.device)
+    dw = torch.empty((plan.tokens, plan.top_k), dtype=torch.float32, device=ys.device)
+    ctx = Context.get(ys.device.index)
+    ctx.check("mr_moe_combine_backward", L.load().mr_moe_combine_backward(
+        ctx.handle, dout.data_ptr(), _stride(dout), ys.data_ptr(), _stride(ys),
+        _ROW_DTYPES[ys.dtype], H, weights.data_ptr(), plan._ref, dys.data_ptr(), dw.data_ptr(),
+        _raw_stream(ys.device)))
+    return dys, dw
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, plan):
+        ctx.plan = plan
+        return _dispatch(x, plan)
+
+    @staticmethod
+    def backward(ctx, dxs):
+        return moe_dispatch_backward(dxs, ctx.plan), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ys, weights, plan, base):
+        ctx.plan = plan
+        ctx.save_for_backward(ys, weights)
+        return _combine(ys, weights, plan, base)
+
+    @staticmethod
+    def backward(ctx, dout):
+        ys, weights = ctx.saved_tensors
+        dys = dw = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            dys, dw = moe_combine_backward(dout, ys, weights, ctx.plan)
+        return dys, dw, None, dout if ctx.needs_input_grad[3] else None
+
+
+def moe_dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
+    """``xs[r] = x[order[r] // top_k]`` [tokens * top_k, hidden]; rows without a pair are zero."""
+    if x.requires_grad and torch.is_grad_enabled():
+        return _Dispatch.apply(x, plan)
+    return _dispatch(x, plan)
+
+
+def moe_combine(ys: torch.Tensor, weights: torch.Tensor, plan: SortedTokens,
+                base: torch.Tensor | None = None) -> torch.Tensor:
+    """``out[t] = base[t] + sum_j weights[t, j] * ys[inverse[t, j]]``: fp32 sums in slot order,
+    one rounding to the type of ``ys``. ``base``: rows to add (the shared expert's)."""
+    if torch.is_grad_enabled() and (ys.requires_grad or weights.requires_grad or
+                                    (base is not None and base.requires_grad)):
+        return _Combine.apply(ys, weights, plan, base)
+    return _combine(ys, weights, plan, base)

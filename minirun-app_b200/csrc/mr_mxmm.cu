@@ -86,16 +86,17 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
   p.nstages = (int)((w->in_features + kMmK - 1) / kMmK);
   p.mtiles = (int)((w->out_features + kMmRows - 1) / kMmRows);
   p.out_f32 = out_dtype == MR_DTYPE_F32;
-  p.wide_scales =
+  const bool wide =
       p.groups % 16 == 0 && addr(w->scales) % 16 == 0 && addr(a->scales) % 16 == 0;
   // Tile width: twice an expert's mean rows, so that few experts need a
   // second tile; narrow tiles leave room for a deeper ring.
   const int64_t mean = plan ? (rows + p.E - 1) / p.E : rows;
   const int64_t want = plan ? std::min(rows, 2 * mean) : rows;
   p.ntile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : kMmMaxN;
-  p.box = p.order ? 1 : std::min(p.ntile, 32);
-  const int fixed = mm_fixed_bytes(p.E);
-  p.nst = std::min(12, (kMmSmem - fixed) / mm_stage_bytes(p.ntile));
+  p.box = p.order ? 1 : p.ntile > 32 ? p.ntile / 2 : p.ntile;  // at most two copies a stage
+  const int fixed = mm_fixed_bytes(p.E, p.ntile);
+  p.nst = std::min((512 - 2 * p.ntile) / mm_sf_cols(p.ntile),
+                   (kMmSmem - fixed) / mm_stage_bytes(p.ntile));
   const int smem = fixed + p.nst * mm_stage_bytes(p.ntile);
 
   MmMaps maps;
@@ -109,10 +110,11 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
     return fail(ctx, MR_ERR_UNSUPPORTED, "the product has more than 2^31 tiles");
   const int grid = (int)std::min<int64_t>(ctx->sm_count, tiles);
   cudaError_t e = set_device(ctx);
+  auto* kernel = wide ? mxmm_kernel<true> : mxmm_kernel<false>;
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(mxmm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmSmem);
   if (e == cudaSuccess)
-    e = launch_pdl(mxmm_kernel, dim3(grid), dim3(kMmThreads), smem,
+    e = launch_pdl(kernel, dim3(grid), dim3(kMmThreads + (p.order ? 32 * kMmGatherWarps : 0)), smem,
                    reinterpret_cast<cudaStream_t>(stream), p, maps);
   return cuda_check(ctx, e, "MXFP4 product");
 }

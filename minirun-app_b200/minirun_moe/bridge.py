@@ -113,8 +113,8 @@ def _stream() -> int:
 
 
 def _raw_stream(device: torch.device) -> int:
-    """The current stream of a tensor's device."""
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of a tensor's device (without a Stream object: 0.1 us, not 2)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _ptr(t: torch.Tensor | None) -> C.c_void_p:

@@ -58,14 +58,16 @@ def mxfp4_quantize(x: torch.Tensor, values: bool = False):
             f"inFeatures {width} is not a multiple of groupSize 32; partial final groups are "
             "not supported")
     dev = x.device
-    packed = torch.empty(shape[:-1] + (width // 8,), dtype=torch.int32, device=dev)
-    scales = torch.empty(shape[:-1] + (width // 32,), dtype=torch.uint8, device=dev)
-    out = torch.empty(shape, dtype=x.dtype, device=dev) if values else None
+    packed = x.new_empty(shape[:-1] + (width // 8,), dtype=torch.int32)
+    scales = x.new_empty(shape[:-1] + (width // 32,), dtype=torch.uint8)
+    out = x.new_empty(shape) if values else None
     ctx = Context.get(dev.index)
     stride = max(x.stride(0), width) if x.dim() == 2 else width
-    ctx.check("mr_mxfp4_quantize", L.load().mr_mxfp4_quantize(
+    st = L.load().mr_mxfp4_quantize(
         ctx.handle, x.data_ptr(), _IN_DTYPES[x.dtype], rows, width, stride, packed.data_ptr(),
-        scales.data_ptr(), None if out is None else out.data_ptr(), _raw_stream(dev)))
+        scales.data_ptr(), None if out is None else out.data_ptr(), _raw_stream(dev))
+    if st:
+        ctx.check("mr_mxfp4_quantize", st)
     experts = shape[0] if x.dim() == 3 else None
     q = _weights_of(packed, scales, shape[-2], width, experts)
     return (q, out) if values else q
@@ -80,13 +82,15 @@ def mxfp4_quantize_swiglu(gate_up: torch.Tensor, limit: float = 0.0) -> MXFP4Wei
             f"gate_up must be [rows, 2 * inter] with inter a multiple of 32, got {list(x.shape)}")
     rows, width = x.shape[0], x.shape[1] // 2
     dev = x.device
-    packed = torch.empty((rows, width // 8), dtype=torch.int32, device=dev)
-    scales = torch.empty((rows, width // 32), dtype=torch.uint8, device=dev)
+    packed = x.new_empty((rows, width // 8), dtype=torch.int32)
+    scales = x.new_empty((rows, width // 32), dtype=torch.uint8)
     ctx = Context.get(dev.index)
-    ctx.check("mr_mxfp4_quantize_swiglu", L.load().mr_mxfp4_quantize_swiglu(
+    st = L.load().mr_mxfp4_quantize_swiglu(
         ctx.handle, x.data_ptr(), _IN_DTYPES[x.dtype], rows, width,
         max(x.stride(0), 2 * width), limit, packed.data_ptr(), scales.data_ptr(),
-        _raw_stream(dev)))
+        _raw_stream(dev))
+    if st:
+        ctx.check("mr_mxfp4_quantize_swiglu", st)
     return _weights_of(packed, scales, rows, width, None)
 
 
@@ -110,10 +114,12 @@ def mxfp4_scaled_mm(a: MXFP4Weights, w: MXFP4Weights,
     if w.experts is not None:
         raise MXFP4BridgeError("mxfp4_scaled_mm needs a single matrix; use mxfp4_grouped_mm")
     dev = a.packed.device
-    out = torch.empty((a.out_features, w.out_features), dtype=out_dtype, device=dev)
+    out = a.packed.new_empty((a.out_features, w.out_features), dtype=out_dtype)
     ctx = Context.get(dev.index)
-    ctx.check("mr_mxfp4_scaled_mm", L.load().mr_mxfp4_scaled_mm(
-        ctx.handle, C.byref(a.desc()), C.byref(w.desc()), dt, out.data_ptr(), _raw_stream(dev)))
+    st = L.load().mr_mxfp4_scaled_mm(ctx.handle, C.byref(a.desc()), C.byref(w.desc()), dt,
+                                     out.data_ptr(), _raw_stream(dev))
+    if st:
+        ctx.check("mr_mxfp4_scaled_mm", st)
     return out
 
 
@@ -138,9 +144,10 @@ def mxfp4_grouped_mm(a: MXFP4Weights, w: MXFP4Weights, plan: SortedTokens,
     dev = a.packed.device
     if plan.device != dev:
         raise MXFP4BridgeError(f"a is on {dev}, the sorted tokens on {plan.device}")
-    out = torch.empty((plan.rows, w.out_features), dtype=out_dtype, device=dev)
+    out = a.packed.new_empty((plan.rows, w.out_features), dtype=out_dtype)
     ctx = Context.get(dev.index)
-    ctx.check("mr_mxfp4_grouped_mm", L.load().mr_mxfp4_grouped_mm(
-        ctx.handle, C.byref(a.desc()), C.byref(w.desc()), plan._ref, int(by_token), dt,
-        out.data_ptr(), _raw_stream(dev)))
+    st = L.load().mr_mxfp4_grouped_mm(ctx.handle, C.byref(a.desc()), C.byref(w.desc()), plan._ref,
+                                      int(by_token), dt, out.data_ptr(), _raw_stream(dev))
+    if st:
+        ctx.check("mr_mxfp4_grouped_mm", st)
     return out

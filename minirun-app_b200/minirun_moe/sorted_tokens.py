@@ -44,20 +44,45 @@ class SortedTokens:
                 raise AffineBridgeError("sorted tokens are contiguous CUDA int32 tensors")
             if t.device != order.device:
                 raise AffineBridgeError("sorted tokens must be on one device")
-        self._fill(order, inverse, offsets, experts)
+        self._views = (order, inverse, offsets)
+        self._fill(order.data_ptr(), inverse.data_ptr(), offsets.data_ptr(), inverse.shape[0],
+                   inverse.shape[1], experts, order.device)
 
-    def _fill(self, order, inverse, offsets, experts):
-        self.order, self.inverse, self.offsets = order, inverse, offsets
-        self.experts = experts
-        self.tokens, self.top_k = inverse.shape
-        self.device = order.device
-        self._c = L.mr_sorted(order.data_ptr(), inverse.data_ptr(), offsets.data_ptr(),
-                              self.tokens, self.top_k, experts)
+    def _fill(self, order, inverse, offsets, tokens, top_k, experts, device):
+        self.tokens, self.top_k, self.experts = tokens, top_k, experts
+        self.rows = tokens * top_k
+        self.device = device
+        self._c = L.mr_sorted(order, inverse, offsets, tokens, top_k, experts)
         self._ref = C.byref(self._c)
 
+    @classmethod
+    def _of(cls, mem: torch.Tensor, tokens: int, top_k: int, experts: int) -> "SortedTokens":
+        """The plan in one buffer (order, inverse, offsets); its views are made when asked for."""
+        s = cls.__new__(cls)
+        s._mem, s._views = mem, None
+        at, P = mem.data_ptr(), 4 * tokens * top_k
+        s._fill(at, at + P, at + 2 * P, tokens, top_k, experts, mem.device)
+        return s
+
+    def _split(self):
+        if self._views is None:
+            P, k = self.rows, self.top_k
+            m = self._mem
+            self._views = (m.as_strided((P,), (1,), 0), m.as_strided((self.tokens, k), (k, 1), P),
+                           m.as_strided((self.experts + 1,), (1,), 2 * P))
+        return self._views
+
     @property
-    def rows(self) -> int:
-        return self.tokens * self.top_k
+    def order(self) -> torch.Tensor:
+        return self._split()[0]
+
+    @property
+    def inverse(self) -> torch.Tensor:
+        return self._split()[1]
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        return self._split()[2]
 
 
 def moe_sort(ids: torch.Tensor, experts: int) -> SortedTokens:
@@ -71,18 +96,13 @@ def moe_sort(ids: torch.Tensor, experts: int) -> SortedTokens:
     if not ids.is_contiguous():
         ids = ids.contiguous()
     T, k = ids.shape
-    dev = ids.device
-    P = T * k
-    # one allocation: inverse, order, offsets
-    mem = torch.empty((2 * P + max(experts, 0) + 1,), dtype=torch.int32, device=dev)
-    order, inverse, offsets = mem[:P], mem[P:2 * P].view(T, k), mem[2 * P:]
-    ctx = Context.get(dev.index)
-    at = mem.data_ptr()
-    ctx.check("mr_moe_sort", L.load().mr_moe_sort(
-        ctx.handle, ids.data_ptr(), T, k, experts, at, at + 4 * P, at + 8 * P,
-        _raw_stream(dev)))
-    s = SortedTokens.__new__(SortedTokens)
-    s._fill(order, inverse, offsets, experts)
+    mem = ids.new_empty((2 * T * k + max(experts, 0) + 1,))
+    s = SortedTokens._of(mem, T, k, experts)
+    c, ctx = s._c, Context.get(s.device.index)
+    st = L.load().mr_moe_sort(ctx.handle, ids.data_ptr(), T, k, experts, c.order, c.inverse,
+                              c.offsets, _raw_stream(s.device))
+    if st:
+        ctx.check("mr_moe_sort", st)
     return s
 
 
@@ -104,7 +124,8 @@ def _stride(t: torch.Tensor) -> int:
 
 
 def _weights(w: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
-    if w.shape != plan.inverse.shape or w.dtype != torch.float32 or w.device != plan.device:
+    if w.shape != (plan.tokens, plan.top_k) or w.dtype != torch.float32 or (
+            w.device != plan.device):
         raise AffineBridgeError(
             f"weights must be [{plan.tokens}, {plan.top_k}] float32 on {plan.device}, got "
             f"{list(w.shape)} {w.dtype} on {w.device}")
@@ -114,11 +135,12 @@ def _weights(w: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
 def _dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     x = _rows("x", x, plan.tokens, plan)
     H = x.shape[1]
-    xs = torch.empty((plan.rows, H), dtype=x.dtype, device=x.device)
-    ctx = Context.get(x.device.index)
-    ctx.check("mr_moe_dispatch", L.load().mr_moe_dispatch(
-        ctx.handle, x.data_ptr(), _ROW_DTYPES[x.dtype], _stride(x), H, plan._ref,
-        xs.data_ptr(), _raw_stream(x.device)))
+    xs = x.new_empty((plan.rows, H))
+    ctx = Context.get(plan.device.index)
+    st = L.load().mr_moe_dispatch(ctx.handle, x.data_ptr(), _ROW_DTYPES[x.dtype], _stride(x), H,
+                                  plan._ref, xs.data_ptr(), _raw_stream(plan.device))
+    if st:
+        ctx.check("mr_moe_dispatch", st)
     return xs
 
 
@@ -126,11 +148,13 @@ def moe_dispatch_backward(dxs: torch.Tensor, plan: SortedTokens) -> torch.Tensor
     """Gradient of ``moe_dispatch``: ``dx[t] = sum_j dxs[inverse[t, j]]``, fp32 sums."""
     dxs = _rows("dxs", dxs, plan.rows, plan)
     H = dxs.shape[1]
-    dx = torch.empty((plan.tokens, H), dtype=dxs.dtype, device=dxs.device)
-    ctx = Context.get(dxs.device.index)
-    ctx.check("mr_moe_dispatch_backward", L.load().mr_moe_dispatch_backward(
-        ctx.handle, dxs.data_ptr(), _ROW_DTYPES[dxs.dtype], _stride(dxs), H, plan._ref,
-        dx.data_ptr(), _raw_stream(dxs.device)))
+    dx = dxs.new_empty((plan.tokens, H))
+    ctx = Context.get(plan.device.index)
+    st = L.load().mr_moe_dispatch_backward(ctx.handle, dxs.data_ptr(), _ROW_DTYPES[dxs.dtype],
+                                           _stride(dxs), H, plan._ref, dx.data_ptr(),
+                                           _raw_stream(plan.device))
+    if st:
+        ctx.check("mr_moe_dispatch_backward", st)
     return dx
 
 
@@ -144,12 +168,13 @@ def _combine(ys, weights, plan, base) -> torch.Tensor:
                 f"base must be [{plan.tokens}, {H}] {ys.dtype} on {ys.device}, got "
                 f"{list(base.shape)} {base.dtype} on {base.device}")
         base = base.contiguous()
-    out = torch.empty((plan.tokens, H), dtype=ys.dtype, device=ys.device)
-    ctx = Context.get(ys.device.index)
-    ctx.check("mr_moe_combine", L.load().mr_moe_combine(
-        ctx.handle, ys.data_ptr(), _ROW_DTYPES[ys.dtype], _stride(ys), H, weights.data_ptr(),
-        None if base is None else base.data_ptr(), plan._ref, out.data_ptr(),
-        _raw_stream(ys.device)))
+    out = ys.new_empty((plan.tokens, H))
+    ctx = Context.get(plan.device.index)
+    st = L.load().mr_moe_combine(ctx.handle, ys.data_ptr(), _ROW_DTYPES[ys.dtype], _stride(ys), H,
+                                 weights.data_ptr(), None if base is None else base.data_ptr(),
+                                 plan._ref, out.data_ptr(), _raw_stream(plan.device))
+    if st:
+        ctx.check("mr_moe_combine", st)
     return out
 
 
@@ -163,13 +188,15 @@ def moe_combine_backward(dout: torch.Tensor, ys: torch.Tensor, weights: torch.Te
         raise AffineBridgeError(
             f"dout must be [{plan.tokens}, {H}] {ys.dtype}, got {list(dout.shape)} {dout.dtype}")
     weights = _weights(weights, plan)
-    dys = torch.empty((plan.rows, H), dtype=ys.dtype, device=ys.device)
-    dw = torch.empty((plan.tokens, plan.top_k), dtype=torch.float32, device=ys.device)
-    ctx = Context.get(ys.device.index)
-    ctx.check("mr_moe_combine_backward", L.load().mr_moe_combine_backward(
+    dys = ys.new_empty((plan.rows, H))
+    dw = weights.new_empty((plan.tokens, plan.top_k))
+    ctx = Context.get(plan.device.index)
+    st = L.load().mr_moe_combine_backward(
         ctx.handle, dout.data_ptr(), _stride(dout), ys.data_ptr(), _stride(ys),
         _ROW_DTYPES[ys.dtype], H, weights.data_ptr(), plan._ref, dys.data_ptr(), dw.data_ptr(),
-        _raw_stream(ys.device)))
+        _raw_stream(plan.device))
+    if st:
+        ctx.check("mr_moe_combine_backward", st)
     return dys, dw
 
 

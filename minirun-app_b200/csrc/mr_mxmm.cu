@@ -84,7 +84,6 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
   p.top_k = plan ? plan->top_k : 1;
   p.groups = (int)(w->in_features / 32);
   p.nstages = (int)((w->in_features + kMmK - 1) / kMmK);
-  p.mtiles = (int)((w->out_features + kMmRows - 1) / kMmRows);
   p.out_f32 = out_dtype == MR_DTYPE_F32;
   const bool wide =
       p.groups % 16 == 0 && addr(w->scales) % 16 == 0 && addr(a->scales) % 16 == 0;
@@ -93,11 +92,13 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
   const int64_t mean = plan ? (rows + p.E - 1) / p.E : rows;
   const int64_t want = plan ? std::min(rows, 2 * mean) : rows;
   p.ntile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : kMmMaxN;
-  p.box = p.order ? 1 : p.ntile > 32 ? p.ntile / 2 : p.ntile;  // at most two copies a stage
+  const int cg = p.ntile > 64 ? 2 : 1;
+  p.mtiles = (int)((w->out_features + kMmRows * cg - 1) / (kMmRows * cg));
+  p.box = p.order ? 1 : p.ntile > 32 ? p.ntile / 2 : p.ntile;
   const int fixed = mm_fixed_bytes(p.E, p.ntile);
   p.nst = std::min((512 - 2 * p.ntile) / mm_sf_cols(p.ntile),
-                   (kMmSmem - fixed) / mm_stage_bytes(p.ntile));
-  const int smem = fixed + p.nst * mm_stage_bytes(p.ntile);
+                   (kMmSmem - fixed) / mm_stage_bytes(p.ntile, cg));
+  const int smem = fixed + p.nst * mm_stage_bytes(p.ntile, cg);
 
   MmMaps maps;
   const int64_t bytes = w->in_features / 2;
@@ -108,14 +109,30 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
   const int64_t tiles = (std::min<int64_t>(p.E, rows) + rows / p.ntile) * p.mtiles;
   if (tiles > INT32_MAX)
     return fail(ctx, MR_ERR_UNSUPPORTED, "the product has more than 2^31 tiles");
-  const int grid = (int)std::min<int64_t>(ctx->sm_count, tiles);
+  const int grid = (int)std::min<int64_t>(ctx->sm_count / cg, tiles) * cg;
+  const int threads = kMmThreads + (p.order ? 32 * kMmGatherWarps : 0);
+  auto* kernel = cg == 1 ? (wide ? mxmm_kernel<true, 1> : mxmm_kernel<false, 1>)
+                         : (wide ? mxmm_kernel<true, 2> : mxmm_kernel<false, 2>);
   cudaError_t e = set_device(ctx);
-  auto* kernel = wide ? mxmm_kernel<true> : mxmm_kernel<false>;
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmSmem);
-  if (e == cudaSuccess)
-    e = launch_pdl(kernel, dim3(grid), dim3(kMmThreads + (p.order ? 32 * kMmGatherWarps : 0)), smem,
-                   reinterpret_cast<cudaStream_t>(stream), p, maps);
+  if (e == cudaSuccess) {
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cg;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, kernel, p, maps);
+  }
   return cuda_check(ctx, e, "MXFP4 product");
 }
 

@@ -5,19 +5,24 @@
 //
 // over blocks b of 32 elements; tcgen05.mma kind::mxf4 multiplies e2m1 codes
 // and both e8m0 scales exactly and sums in fp32. A tile is 128 weight rows
-// (the M side, one TMEM lane each) by up to `ntile` activation rows (the N
-// side, one TMEM column each): weight matrices are whole multiples of 128
-// rows while an expert's rows are any number, and N steps by 16.
+// a CTA (the M side, one TMEM lane each) by up to `ntile` activation rows
+// (the N side, one TMEM column each): weight matrices are whole multiples of
+// 128 rows while an expert's rows are any number, and N steps by 16.
 //
-// One CTA per SM loops over tiles (expert's row tile x 128 weight rows, the
-// weight rows fastest, so that CTAs working side by side share activations).
-// Per stage of 256 elements (128 bytes of codes a row):
-//   - warp 0: TMA loads of both operands' codes (128-byte swizzle) into the
-//     ring;
+// CG = 1: one CTA a tile. CG = 2: a cluster of two CTAs a tile of 256 weight
+// rows; each loads its own 128 rows and half of the activations, and the
+// leader's MMAs (cta_group::2) read both halves: per MMA a CTA takes 28 KB
+// from L2 instead of 40.
+//
+// Persistent CTAs (or pairs) loop over tiles (expert's row tile x weight
+// rows, the weight rows fastest, so that CTAs working side by side share
+// activations). Per stage of 512 elements (256 bytes of codes a row, as two
+// pieces of the 128 that the swizzle spans):
+//   - warp 0: TMA loads of the codes (128-byte swizzle) into the ring;
 //   - warps 12-15, by_token: the activations' codes instead, by TMA gathers of
-//     four rows (48 a stage are more than one warp issues in a stage's time);
-//   - warps 2 and 3: the exponents of weights / activations, 16 a row (two
-//     stages) at a time, from global to shared memory;
+//     four rows (58 cycles each to issue: more than one warp can in a stage);
+//   - warps 2 and 3: the exponents of weights / activations, 16 a row, from
+//     global to shared memory;
 //   - warps 8-11: the exponents from there into tensor memory, each warp its
 //     lane quadrant (the tensor core reads the exponents of 32 rows a column,
 //     in every quadrant). No proxy fence is on this way: one in the loading
@@ -36,21 +41,30 @@
 // runs to its end on garbage, drains its copies and MMAs, frees its TMEM.
 #pragma once
 
+#include <cooperative_groups.h>
+
 #include "mr_gemv_umma.cuh"
 
 namespace mr {
 
-constexpr int kMmRows = 128;    // weight rows of a tile (MMA M)
-constexpr int kMmK = 256;       // elements of a stage
-constexpr int kMmMaxN = 192;      // activation rows of a tile: two accumulators and five
-                                // slots of exponents fit the 512 TMEM columns
-constexpr int kMmThreads = 384;   // plus the gather warps
+constexpr int kMmRows = 128;     // weight rows of a CTA (MMA M = 128 CG)
+constexpr int kMmK = 512;        // elements of a stage: with 256 the waits of one, 50-200
+                                 // cycles each, took longer than its MMAs
+constexpr int kMmMaxN = 176;     // activation rows of a tile: two accumulators and three
+                                 // slots of exponents fit the 512 TMEM columns
+constexpr int kMmB = (kMmMaxN + 31) / 32;
+constexpr int kMmThreads = 384;  // plus the gather warps
 constexpr int kMmGatherWarps = 4;
-constexpr int kMmGathers = kMmMaxN / 4 / kMmGatherWarps;  // a warp's in a stage, at most
-constexpr int kMmABytes = kMmRows * 128;
-constexpr int kMmRaw = 3;  // slots of the exponents' ring in shared memory, two stages each
-// TMEM columns of one stage's exponents: 4 a word of A, 4 a word and 128 rows of B.
-MR_DEVICE __host__ constexpr int mm_sf_cols(int ntile) { return 8 + 8 * ((ntile + 127) / 128); }
+constexpr int kMmAPiece = kMmRows * 128;
+constexpr int kMmRaw = 3;  // slots of the exponents' ring in shared memory
+
+// The MMAs' N, and a tile's width, step by 16.
+MR_DEVICE __host__ constexpr int mm_round(int n) { return (n + 15) & ~15; }
+// TMEM columns of a word (four exponents a row) of B, and of a stage.
+MR_DEVICE __host__ constexpr int mm_sf_word(int ntile) { return 4 * ((ntile + 127) / 128); }
+MR_DEVICE __host__ constexpr int mm_sf_cols(int ntile) { return 16 + 4 * mm_sf_word(ntile); }
+// Rows of exponents of one slot in shared memory.
+MR_DEVICE __host__ constexpr int mm_raw_rows(int ntile) { return kMmRows + (ntile + 31) / 32 * 32; }
 
 struct MmParams {
   const uint8_t* w_scales;  // [E, out, in / 32]
@@ -61,9 +75,9 @@ struct MmParams {
   unsigned* error;
   int64_t rows, arows, out_features;
   int E, top_k;
-  int groups;               // in / 32
+  int groups;           // in / 32
   int nstages, mtiles;
-  int ntile, box, nst;      // tile width, rows of an activation box, ring stages
+  int ntile, box, nst;  // tile width, rows of an activation box, ring stages
   int out_f32;
 };
 struct MmMaps {
@@ -71,36 +85,87 @@ struct MmMaps {
 };
 
 // Shared memory: ring of codes, ring of exponents, barriers, group table.
-MR_DEVICE __host__ constexpr int mm_raw_bytes(int ntile) { return (kMmRows + ntile) * 16; }
-inline int mm_stage_bytes(int ntile) { return kMmABytes + ntile * 128; }
+inline int mm_stage_bytes(int ntile, int cg) { return 2 * (kMmAPiece + ntile / cg * 128); }
 inline int mm_fixed_bytes(int E, int ntile) {
-  return 1024 + kMmRaw * mm_raw_bytes(ntile) + 512 + 2 * (E + 1) * 4;
+  return 1024 + kMmRaw * mm_raw_rows(ntile) * 16 + 768 + 2 * (E + 1) * 4;
 }
+
+// ------------------------------------------------------------ instructions
 
 // True in one lane of a converged warp.
 MR_DEVICE bool elect_one() {
   uint32_t on;
-  asm volatile("{ .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p; }" : "=r"(on));
+  asm volatile("{ .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p; }"
+               : "=r"(on));
   return on != 0;
 }
-// D[128 x N] (+)= A . B^T with scales; both operands by shared descriptors.
+MR_DEVICE uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+template <int CG>
+MR_DEVICE void mm_tmem_alloc(uint32_t* dst) {
+  if constexpr (CG == 1) {
+    tmem_alloc(dst, 512);
+    tmem_relinquish();
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_u32(dst))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+}
+template <int CG>
+MR_DEVICE void mm_tmem_dealloc() {
+  if constexpr (CG == 1)
+    tmem_dealloc(0, 512);
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(0u) : "memory");
+}
+// Arrive on `bar` (of both CTAs of a pair) when this thread's MMAs are done.
+template <int CG>
+MR_DEVICE void mm_commit(uint64_t* bar) {
+  if constexpr (CG == 1)
+    tc_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// D[128 CG x N] (+)= A . B^T with scales; both operands by shared descriptors.
+template <int CG>
 MR_DEVICE void tc_mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                            uint32_t sfa, uint32_t sfb, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
-      "[%5], p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
-      : "memory");
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
+        "[%5], p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
+        "[%5], p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
 }
-// wait_bounded with its first look at the barrier outside the loop. One lane
-// of a warp waits so only where the others have left; elsewhere all lanes
-// wait together. (Lanes parked at a warp barrier made every branch of the
-// running one slow: 185-280 cycles for a wait that is already over, here 53.)
-MR_DEVICE void wait_mbar(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                         unsigned* error) {
-  if (!mbar_try_wait(bar, parity)) wait_bounded(bar, parity, abort_flag, error);
+// kind::mxf4, e2m1 x e2m1, e8m0 scales, M = 128 CG; `half`: which two of a
+// word's four exponents (both operands).
+template <int CG>
+MR_DEVICE uint32_t umma_idesc_mxf4(int n, uint32_t half) {
+  return (half << 5)                   // B exponents: id 0 or 2 at bits 4-5
+         | (1u << 7) | (1u << 10)      // A, B: e2m1
+         | ((uint32_t)(n >> 3) << 17)  // N / 8
+         | (1u << 23)                  // exponents: e8m0
+         | ((uint32_t)CG << 27)        // M / 128
+         | (half << 30);               // A exponents: id at bits 29-30
 }
 // Four consecutive TMEM columns of this thread's lane.
 MR_DEVICE void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -108,17 +173,6 @@ MR_DEVICE void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint
                "r"(a), "r"(b), "r"(c), "r"(d)
                : "memory");
 }
-// kind::mxf4, e2m1 x e2m1, e8m0 scales, M = 128; `half`: which two of a
-// word's four exponents (both operands).
-MR_DEVICE uint32_t umma_idesc_mxf4(int n, uint32_t half) {
-  return (half << 5)                   // B exponents: id 0 or 2 at bits 4-5
-         | (1u << 7) | (1u << 10)      // A, B: e2m1
-         | ((uint32_t)(n >> 3) << 17)  // N / 8
-         | (1u << 23)                  // exponents: e8m0
-         | (1u << 27)                  // M / 128
-         | (half << 30);               // A exponents: id at bits 29-30
-}
-
 // Four rows (y) of 128 bytes at column x.
 MR_DEVICE void tma_gather4(void* dst, const CUtensorMap* map, int x, const int4& y,
                            uint64_t* bar) {
@@ -129,27 +183,62 @@ MR_DEVICE void tma_gather4(void* dst, const CUtensorMap* map, int x, const int4&
       "r"(smem_u32(bar))
       : "memory");
 }
+// Arrive on the barrier at this place in the CTA of rank `to`. Relaxed: what
+// it tells of is complete by itself (tensor memory after tcgen05.wait, copies
+// after their barrier, MMAs after their commit) and no plain store is handed
+// over; a release at cluster scope took 500-2000 cycles.
+template <int CG>
+MR_DEVICE void mm_arrive(uint64_t* bar, uint32_t to, uint32_t rank) {
+  if (CG == 1 || to == rank) {
+    mbar_arrive(bar);
+  } else {
+    asm volatile(
+        "{ .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n"
+        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [r]; }" ::"r"(smem_u32(bar)),
+        "r"(to)
+        : "memory");
+  }
+}
+// wait_bounded as one look at the barrier and a call where that is not
+// enough: sixteen warps run different code, and its size costs each of them.
+// One lane of a warp waits alone only where the others have left; elsewhere
+// all lanes wait together. (Lanes parked at a warp barrier made every branch
+// of the running one slow: 185-280 cycles for a wait that is already over,
+// against 53.)
+__device__ __noinline__ void wait_called(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                         unsigned* error) {
+  wait_bounded(bar, parity, abort_flag, error);
+}
+MR_DEVICE void wait_mbar(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                         unsigned* error) {
+  if (__builtin_expect(!mbar_try_wait(bar, parity), 0)) wait_called(bar, parity, abort_flag, error);
+}
 
-// An expert's n rows in tiles of equal width, a multiple of 16: as few as
-// ntile allows, none empty.
+// ------------------------------------------------------------------- tiles
+
+// An expert's n rows in tiles of equal width: as few as ntile allows, none
+// empty.
 MR_DEVICE int mm_width(int n, int ntile) {
   const int c = (n + ntile - 1) / ntile;
-  return c > 0 ? ((n + c - 1) / c + 15) & ~15 : 16;
+  return c > 0 ? mm_round((n + c - 1) / c) : 16;
 }
 MR_DEVICE int mm_tiles(int n, int ntile) {
   const int w = mm_width(n, ntile);
   return (n + w - 1) / w;
 }
 
-// Walks the CTA's tiles in order: item -> expert, rows and weight rows.
+// Walks the CTA's (or pair's) tiles in order: item -> expert, rows, and the
+// CTA's weight rows.
+template <int CG>
 struct MmWalk {
-  const int* goff;    // [E + 1] first row of each expert
-  const int* gtile;   // [E + 1] first row tile of each expert
+  const int* goff;   // [E + 1] first row of each expert
+  const int* gtile;  // [E + 1] first row tile of each expert
   int mtiles, ntile;
+  int m_in;          // the CTA's first row in a tile
   int e = 0, row0 = 0, n = 0, m0 = 0;
   MR_DEVICE void at(int item) {
     const int t = item / mtiles;
-    m0 = (item - t * mtiles) * kMmRows;
+    m0 = (item - t * mtiles) * (kMmRows * CG) + m_in;
     while (gtile[e + 1] <= t) ++e;
     const int all = goff[e + 1] - goff[e];
     const int w = mm_width(all, ntile);
@@ -158,6 +247,8 @@ struct MmWalk {
     n = min(w, all - first);
   }
 };
+
+// ------------------------------------------------------------ exponents
 
 // The token row that sorted row r takes its activations from.
 MR_DEVICE int64_t mm_act_row(const MmParams& p, int64_t r) {
@@ -178,7 +269,7 @@ MR_DEVICE uint4 mm_ldg16(const uint8_t* at, const uint8_t* lo, const uint8_t* hi
 }
 
 // One warp's exponents: rows lane + 32 i (i < NB) of a tile's weights or
-// activations, 16 a row (two stages) at a time. WIDE: every row is made of
+// activations, 16 a row (a stage's). WIDE: every row is made of
 // aligned 16-byte pieces. Otherwise a row starts at any byte and 16 exponents
 // lie in one or two aligned pieces, shifted together when they are used.
 template <int NB, bool WIDE>
@@ -230,18 +321,17 @@ struct MmScaleRegs {
   }
 };
 
-// Exponents from global to shared memory, loaded one or two pairs of stages
-// (also of the next tile) ahead of their use: the loads' latency stays out of the
+// Exponents from global to shared memory, loaded one or two stages (also of
+// the next tile) ahead of their use: the loads' latency stays out of the
 // pipeline. A slot holds 16 bytes a row. Every lane of the warp.
-template <int NB, bool WIDE, bool IS_A>
-MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk& walk, int lane, int n_items,
-                              uint4* raw, uint64_t* rfull, uint64_t* rempty,
-                              volatile int* flags) {
-  const int npairs = (p.nstages + 1) / 2;
-  const int slot_rows = kMmRows + p.ntile;
+template <int NB, bool WIDE, bool IS_A, int CG>
+MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lane, int first,
+                              int stride, int n_items, uint4* raw, uint64_t* rfull,
+                              uint64_t* rempty, volatile int* flags) {
+  const int slot_rows = mm_raw_rows(p.ntile);
   const uint8_t* lo = IS_A ? p.w_scales : p.a_scales;
   const uint8_t* hi = lo + (IS_A ? (int64_t)p.E * p.out_features : p.arows) * p.groups;
-  MmWalk it = walk;
+  MmWalk<CG> it = walk;
   const uint8_t* src[NB];
   auto open = [&](int item) {
     if (item >= n_items) return;
@@ -257,7 +347,7 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk& walk, int lane, i
       src[i] = 32 * i < have ? lo + row * p.groups : nullptr;
     }
   };
-  constexpr int kAhead = WIDE ? 2 : 1;  // registers of two unaligned pairs would spill
+  constexpr int kAhead = WIDE ? 2 : 1;  // registers of two unaligned stages would spill
   MmScaleRegs<NB, WIDE> v[kAhead];
 #pragma unroll
   for (int b = 0; b < kAhead; ++b)
@@ -269,21 +359,21 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk& walk, int lane, i
         v[b].off[i] = 0;
       }
     }
-  int litem = blockIdx.x, lq = 0;  // the pair to load next
+  int litem = first, lq = 0;  // the stage to load next
   open(litem);
   auto load = [&](MmScaleRegs<NB, WIDE>& r) {
     if (litem >= n_items) return;
     r.load(src, lq, p.groups, lo, hi);
-    if (++lq == npairs) {
+    if (++lq == p.nstages) {
       lq = 0;
-      litem += gridDim.x;
+      litem += stride;
       open(litem);
     }
   };
 #pragma unroll
   for (int b = 0; b < kAhead; ++b) load(v[b]);
   uint32_t slot = 0, phase = 0;
-  int item = blockIdx.x, q = 0;  // the pair to hand on next
+  int item = first, q = 0;  // the stage to hand on next
   while (item < n_items) {
 #pragma unroll
     for (int b = 0; b < kAhead; ++b) {
@@ -292,7 +382,7 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk& walk, int lane, i
       uint4* dst = raw + slot * slot_rows + (IS_A ? 0 : kMmRows) + lane;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
-        if (IS_A || 32 * i + lane < p.ntile) dst[32 * i] = v[b].get(i);
+        if (IS_A || 32 * i < p.ntile) dst[32 * i] = v[b].get(i);
       __syncwarp();
       if (lane == 0) mbar_arrive(rfull + slot);
       if (++slot == kMmRaw) {
@@ -300,25 +390,26 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk& walk, int lane, i
         phase ^= 1u;
       }
       load(v[b]);
-      if (++q == npairs) {
+      if (++q == p.nstages) {
         q = 0;
-        item += gridDim.x;
+        item += stride;
       }
     }
   }
 }
 
-template <bool WIDE>
+template <bool WIDE, int CG>
 __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     mxmm_kernel(const MmParams p, const __grid_constant__ MmMaps maps) {
   extern __shared__ char smem_raw[];
   char* smem =
       reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int b_bytes = p.ntile * 128;
+  const int b_piece = p.ntile / CG * 128;
   const int nst = p.nst;
-  char* bring = smem + nst * kMmABytes;
-  uint4* raw = reinterpret_cast<uint4*>(bring + nst * b_bytes);  // [kMmRaw][128 + ntile]
-  uint64_t* full = reinterpret_cast<uint64_t*>(raw + kMmRaw * (kMmRows + p.ntile));  // [nst]
+  char* bring = smem + nst * 2 * kMmAPiece;
+  uint4* raw = reinterpret_cast<uint4*>(bring + nst * 2 * b_piece);  // [kMmRaw][raw rows]
+  uint64_t* lfull = reinterpret_cast<uint64_t*>(raw + kMmRaw * mm_raw_rows(p.ntile));  // [nst]
+  uint64_t* full = lfull + nst;       // [nst] a stage's operands there, of both CTAs
   uint64_t* empty = full + nst;       // [nst]
   uint64_t* rfull = empty + nst;      // [kMmRaw] exponents in shared memory
   uint64_t* rempty = rfull + kMmRaw;  // [kMmRaw] and read from there
@@ -326,16 +417,22 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   uint64_t* dempty = dfull + 2;       // [2]
   uint64_t* drain = dempty + 2;       // every MMA complete
   uint64_t* done = drain + 1;         // every other access of TMEM too
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* bye = done + 1;           // the other CTA needs this one's memory no more
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bye + 1);
   volatile int* flags = reinterpret_cast<volatile int*>(tslot + 1);
   int* scan = reinterpret_cast<int*>(tslot + 2);  // [16] warp sums
   int* goff = scan + 16;
   int* gtile = goff + p.E + 1;
+  // CG = 1: the copies complete on `full` itself
+  uint64_t* cfull = CG == 1 ? full : lfull;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = CG == 1 ? 0 : cluster_rank();
+  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
   if (tid == 0) {
     for (int s = 0; s < nst; ++s) {
-      mbar_init(full + s, 5);  // the copies' bytes, four warps' exponents
+      mbar_init(lfull + s, 1);
+      mbar_init(full + s, CG == 1 ? 5 : 8);  // four warps' exponents a CTA (CG = 1: the copies)
       mbar_init(empty + s, 1);
     }
     for (int s = 0; s < kMmRaw; ++s) {
@@ -344,17 +441,15 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(dfull + b, 1);
-      mbar_init(dempty + b, 4);
+      mbar_init(dempty + b, 4 * CG);
     }
     mbar_init(drain, 1);
     mbar_init(done, 8);
+    mbar_init(bye, 1);
     flags[0] = 0;
     fence_mbar_init();
   }
-  if (warp == 4) {
-    tmem_alloc(tslot, 512);
-    tmem_relinquish();
-  }
+  if (warp == 4) mm_tmem_alloc<CG>(tslot);
   pdl_wait_and_release();
   // the group table: thread i has experts 4i .. 4i+3 (E <= 1024: the first 256 threads)
   {
@@ -396,30 +491,38 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     }
   }
   tc_fence_before();
-  __syncthreads();
+  if constexpr (CG == 1)
+    __syncthreads();
+  else
+    cooperative_groups::this_cluster().sync();  // the other CTA's barriers are there too
   tc_fence_after();
   constexpr uint32_t tbase = 0;  // all 512 columns are this CTA's: they start at 0
   const int n_items = gtile[p.E] * p.mtiles;
-  MmWalk it{goff, gtile, p.mtiles, p.ntile};
+  MmWalk<CG> it{goff, gtile, p.mtiles, p.ntile, (int)rank * kMmRows};
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (!elect_one()) return;
     uint32_t slot = 0, phase = 0, issued = 0;
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+    for (int item = first; item < n_items; item += stride) {
       it.at(item);
       const int y0 = it.e * (int)p.out_features + it.m0;
-      const int boxes = (it.n + p.box - 1) / p.box;
-      const uint32_t bytes =
-          kMmABytes + (p.order ? (it.n + 15) / 16 * 16 : boxes * p.box) * 128;
+      const int half = mm_round(it.n) / CG;  // activation rows of this CTA
+      const int ya = it.row0 + (int)rank * half;
+      const int boxes = (half + p.box - 1) / p.box;
+      const uint32_t bytes = kMmAPiece + (p.order ? half : boxes * p.box) * 128;  // a piece
       for (int st = 0; st < p.nstages; ++st, ++issued) {
+        const int pieces = min(2, (p.groups - st * 16 + 7) / 8);
         wait_mbar(empty + slot, phase ^ 1u, flags, p.error);
-        mbar_arrive_expect_tx(full + slot, bytes);
-        tma_load_2d(smem + slot * kMmABytes, &maps.w, st * 128, y0, full + slot);
-        if (!p.order)
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d(bring + slot * b_bytes + b * p.box * 128, &maps.a, st * 128,
-                        it.row0 + b * p.box, full + slot);
+        mbar_arrive_expect_tx(cfull + slot, pieces * bytes);
+        for (int k = 0; k < pieces; ++k) {
+          const int x = st * 256 + k * 128;
+          tma_load_2d(smem + (2 * slot + k) * kMmAPiece, &maps.w, x, y0, cfull + slot);
+          if (!p.order)
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d(bring + (2 * slot + k) * b_piece + b * p.box * 128, &maps.a, x,
+                          ya + b * p.box, cfull + slot);
+        }
         if (++slot == (uint32_t)nst) {
           slot = 0;
           phase ^= 1u;
@@ -430,122 +533,143 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       // after an abort, let the copies in flight land before exiting
       for (uint32_t j = (issued > (uint32_t)nst ? issued - nst : 0); j < issued; ++j)
         for (uint32_t i = 0; i < kSpinLimit; ++i)
-          if (mbar_try_wait(full + (j % nst), (j / nst) & 1u)) break;
+          if (mbar_try_wait(cfull + (j % nst), (j / nst) & 1u)) break;
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    if (!elect_one()) return;
-    const int sfc = mm_sf_cols(p.ntile), sfw = sfc / 2 - 4;
+    if (rank != 0 || !elect_one()) return;
+    const int sfc = mm_sf_cols(p.ntile), sfw = mm_sf_word(p.ntile);
     const uint32_t a0 = smem_u32(smem), b0 = smem_u32(bring);
     uint32_t slot = 0, phase = 0, t = 0;
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x, ++t) {
+    for (int item = first; item < n_items; item += stride, ++t) {
       it.at(item);
       const uint32_t db = t & 1u;
-      const int nn = (it.n + 15) & ~15;
+      const int nn = mm_round(it.n);
       wait_mbar(dempty + db, ((t >> 1) & 1u) ^ 1u, flags, p.error);
       const uint32_t d_t = db * p.ntile;
       for (int st = 0; st < p.nstages; ++st) {
-        const uint32_t sfa = 2 * p.ntile + slot * sfc, sfb = sfa + 8;
-        const uint32_t at = a0 + slot * kMmABytes, bt = b0 + slot * b_bytes;
+        const uint32_t sfa = 2 * p.ntile + slot * sfc, sfb = sfa + 16;
+        const uint32_t at = a0 + slot * 2 * kMmAPiece, bt = b0 + slot * 2 * b_piece;
         wait_mbar(full + slot, phase, flags, p.error);
         tc_fence_after();
-        // a row's last stage may hold fewer than four steps of 64
-        const int steps = min(4, (p.groups - st * 8 + 1) / 2);
+        // a row's last stage may hold fewer than eight steps of 64
+        const int steps = min(8, (p.groups - st * 16 + 1) / 2);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
+        for (int kk = 0; kk < 8; ++kk)
           if (kk < steps)
-            tc_mma_mxf4(d_t, umma_desc_sw128(at + kk * 32), umma_desc_sw128(bt + kk * 32),
-                        umma_idesc_mxf4(nn, kk & 1), sfa + 4 * (kk >> 1), sfb + sfw * (kk >> 1),
-                        (st | kk) ? 1u : 0u);
-        tc_commit(empty + slot);
+            tc_mma_mxf4<CG>(d_t, umma_desc_sw128(at + (kk >> 2) * kMmAPiece + (kk & 3) * 32),
+                            umma_desc_sw128(bt + (kk >> 2) * b_piece + (kk & 3) * 32),
+                            umma_idesc_mxf4<CG>(nn, kk & 1), sfa + 4 * (kk >> 1),
+                            sfb + sfw * (kk >> 1), (st | kk) ? 1u : 0u);
+        mm_commit<CG>(empty + slot);
         if (++slot == (uint32_t)nst) {
           slot = 0;
           phase ^= 1u;
         }
       }
-      tc_commit(dfull + db);
+      mm_commit<CG>(dfull + db);
     }
-    tc_commit(drain);
+    mm_commit<CG>(drain);
     wait_mbar(drain, 0, flags, p.error);
   } else if (warp < 4) {
     // ------------------------------------------- exponents to shared memory
     if (warp == 2)
-      mm_load_scales<4, WIDE, true>(p, it, lane, n_items, raw, rfull, rempty, flags);
+      mm_load_scales<4, WIDE, true>(p, it, lane, first, stride, n_items, raw, rfull, rempty,
+                                    flags);
     else
-      mm_load_scales<kMmMaxN / 32, WIDE, false>(p, it, lane, n_items, raw, rfull, rempty, flags);
+      mm_load_scales<kMmB, WIDE, false>(p, it, lane, first, stride, n_items, raw, rfull,
+                                                rempty, flags);
   } else if (warp >= 8 && warp < 12) {
     // -------------------------------------------- exponents to tensor memory
     const uint32_t lane_t = tbase + ((uint32_t)((warp & 3) * 32) << 16) + 2 * p.ntile;
-    const int sfc = mm_sf_cols(p.ntile), slot_rows = kMmRows + p.ntile;
+    const int sfc = mm_sf_cols(p.ntile), sfw = mm_sf_word(p.ntile);
+    const int slot_rows = mm_raw_rows(p.ntile);
     uint32_t slot = 0, phase = 0, rslot = 0, rphase = 0;
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
-      for (int st = 0; st < p.nstages; st += 2) {
-        wait_mbar(rfull + rslot, rphase, flags, p.error);
-        const uint4* src = raw + rslot * slot_rows + lane;
-        uint4 a[4], b[8];  // rows lane + 32 i
+    struct Stage {
+      uint4 a[4], b[kMmB];  // rows lane + 32 i
+    };
+    int64_t left =
+        first < n_items ? (int64_t)((n_items - 1 - first) / stride + 1) * p.nstages : 0;
+    auto fetch = [&](Stage& v) {
+      if (left-- <= 0) return;
+      wait_mbar(rfull + rslot, rphase, flags, p.error);
+      const uint4* src = raw + rslot * slot_rows + lane;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = src[32 * i];
+      for (int i = 0; i < 4; ++i) v.a[i] = src[32 * i];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          b[i] = 32 * i + lane < p.ntile ? src[kMmRows + 32 * i] : make_uint4(0, 0, 0, 0);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(rempty + rslot);
-        if (++rslot == kMmRaw) {
-          rslot = 0;
-          rphase ^= 1u;
-        }
+      for (int i = 0; i < kMmB; ++i)
+        v.b[i] = 32 * i < p.ntile ? src[kMmRows + 32 * i] : make_uint4(0, 0, 0, 0);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(rempty + rslot);
+      if (++rslot == kMmRaw) {
+        rslot = 0;
+        rphase ^= 1u;
+      }
+    };
+    auto hand_on = [&](const Stage& v) {
+      wait_mbar(empty + slot, phase ^ 1u, flags, p.error);
+      tc_fence_after();
+      const uint32_t t = lane_t + slot * sfc;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (st + h >= p.nstages) break;
-          wait_mbar(empty + slot, phase ^ 1u, flags, p.error);
-          tc_fence_after();
-          const uint32_t t = lane_t + slot * sfc;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            // word 2 h + w of each row
-            auto word = [&](const uint4& v) {
-              return h == 0 ? (w == 0 ? v.x : v.y) : (w == 0 ? v.z : v.w);
-            };
-            tmem_st4(t + 4 * w, word(a[0]), word(a[1]), word(a[2]), word(a[3]));
-            const uint32_t tb = t + 8 + w * (sfc / 2 - 4);
-            tmem_st4(tb, word(b[0]), word(b[1]), word(b[2]), word(b[3]));
-            if (p.ntile > 128) tmem_st4(tb + 4, word(b[4]), word(b[5]), word(b[6]), word(b[7]));
-          }
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full + slot);
-          if (++slot == (uint32_t)nst) {
-            slot = 0;
-            phase ^= 1u;
-          }
-        }
+      for (int w = 0; w < 4; ++w) {
+        auto word = [&](const uint4& x) { return w == 0 ? x.x : w == 1 ? x.y : w == 2 ? x.z : x.w; };
+        tmem_st4(t + 4 * w, word(v.a[0]), word(v.a[1]), word(v.a[2]), word(v.a[3]));
+        const uint32_t tb = t + 16 + w * sfw;
+        tmem_st4(tb, word(v.b[0]), word(v.b[1]), word(v.b[2]), word(v.b[3]));
+        if (p.ntile > 128) tmem_st4(tb + 4, word(v.b[4]), word(v.b[5]), 0, 0);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      // one warp vouches for the CTA's copies too
+      if (CG == 2 && warp == 8) wait_mbar(lfull + slot, phase, flags, p.error);
+      if (lane == 0) mm_arrive<CG>(full + slot, 0, rank);
+      if (++slot == (uint32_t)nst) {
+        slot = 0;
+        phase ^= 1u;
+      }
+    };
+    Stage v0, v1;  // the next stage is on its way while one is stored
+    int64_t todo = left;
+    fetch(v0);
+    for (; todo > 0; todo -= 2) {
+      fetch(v1);
+      hand_on(v0);
+      if (todo > 1) {
+        fetch(v0);
+        hand_on(v1);
       }
     }
     if (lane == 0) mbar_arrive(done);
   } else if (warp >= 12) {
     // -------------------------------------------------------------- gathers
     if (!elect_one()) return;
+    constexpr int kMine = (kMmMaxN / CG / 4 + kMmGatherWarps - 1) / kMmGatherWarps;  // a piece's
     const int w = warp - 12;
     uint32_t slot = 0, phase = 0;
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+    for (int item = first; item < n_items; item += stride) {
       it.at(item);
-      const int nq = (it.n + 15) / 16 * 4;
-      int4 rows[kMmGathers];  // every kMmGatherWarps-th gather is this warp's
+      const int half = mm_round(it.n) / CG, nq = half / 4;
+      int4 rows[kMine];  // every kMmGatherWarps-th gather is this warp's
 #pragma unroll
-      for (int i = 0; i < kMmGathers; ++i) {
-        const int r0 = it.row0 + 4 * (w + i * kMmGatherWarps), r1 = it.row0 + it.n - 1;
-        // rows past the tile's end repeat its last
-        rows[i] = make_int4((int)mm_act_row(p, min(r0, r1)), (int)mm_act_row(p, min(r0 + 1, r1)),
-                            (int)mm_act_row(p, min(r0 + 2, r1)), (int)mm_act_row(p, min(r0 + 3, r1)));
+      for (int i = 0; i < kMine; ++i) {
+        const int r0 = it.row0 + (int)rank * half + 4 * (w + i * kMmGatherWarps);
+        const int r1 = it.row0 + it.n - 1;  // rows past the tile's end repeat its last
+        rows[i] =
+            make_int4((int)mm_act_row(p, min(r0, r1)), (int)mm_act_row(p, min(r0 + 1, r1)),
+                      (int)mm_act_row(p, min(r0 + 2, r1)), (int)mm_act_row(p, min(r0 + 3, r1)));
       }
       for (int st = 0; st < p.nstages; ++st) {
+        const int pieces = min(2, (p.groups - st * 16 + 7) / 8);
         wait_mbar(empty + slot, phase ^ 1u, flags, p.error);
-        char* dst = bring + slot * b_bytes;
+        for (int k = 0; k < pieces; ++k) {
+          char* dst = bring + (2 * slot + k) * b_piece;
 #pragma unroll
-        for (int i = 0; i < kMmGathers; ++i) {
-          const int q = w + i * kMmGatherWarps;
-          if (q < nq) tma_gather4(dst + q * 512, &maps.a, st * 128, rows[i], full + slot);
+          for (int i = 0; i < kMine; ++i) {
+            const int q = w + i * kMmGatherWarps;
+            if (q < nq)
+              tma_gather4(dst + q * 512, &maps.a, st * 256 + k * 128, rows[i], cfull + slot);
+          }
         }
         if (++slot == (uint32_t)nst) {
           slot = 0;
@@ -557,7 +681,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     // ------------------------------------------------------------- epilogue
     const int q = warp & 3;
     uint32_t t = 0;
-    for (int item = blockIdx.x; item < n_items; item += gridDim.x) {
+    for (int item = first; item < n_items; item += stride, ++t) {
       it.at(item);
       const uint32_t db = t & 1u;
       wait_mbar(dfull + db, (t >> 1) & 1u, flags, p.error);
@@ -581,8 +705,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(dempty + db);
-      ++t;
+      if (lane == 0) mm_arrive<CG>(dempty + db, 0, rank);
     }
     tc_fence_before();
     __syncwarp();
@@ -590,8 +713,18 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     if (warp == 4) {
       wait_mbar(done, 0, flags, p.error);
       wait_mbar(drain, 0, flags, p.error);
+      // the last arrivals at the ring's barriers, which nobody else waits for
+      const int64_t stages = (int64_t)t * p.nstages;
+      for (int s = 0; s < nst && s < stages; ++s)
+        wait_mbar(empty + s, (uint32_t)((stages - 1 - s) / nst) & 1u, flags, p.error);
       tc_fence_after();
-      tmem_dealloc(tbase, 512);
+      mm_tmem_dealloc<CG>();
+      if constexpr (CG == 2) {
+        // this CTA's arrivals at the other are all made, and the MMAs that
+        // read this one's memory done: leave when the other says the same
+        if (lane == 0) mm_arrive<CG>(bye, rank ^ 1u, rank);
+        wait_mbar(bye, 0, flags, p.error);
+      }
     }
     // rows without a pair
     const int64_t z0 = (int64_t)goff[p.E] * p.out_features, z1 = p.rows * p.out_features;

@@ -167,11 +167,28 @@ MR_DEVICE uint32_t umma_idesc_mxf4(int n, uint32_t half) {
          | ((uint32_t)CG << 27)        // M / 128
          | (half << 30);               // A exponents: id at bits 29-30
 }
-// Four consecutive TMEM columns of this thread's lane.
-MR_DEVICE void tmem_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr),
-               "r"(a), "r"(b), "r"(c), "r"(d)
-               : "memory");
+// Sixteen consecutive TMEM columns of this thread's lane.
+MR_DEVICE void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+MR_DEVICE uint32_t word_of(const uint4& x, int w) {
+  return w == 0 ? x.x : w == 1 ? x.y : w == 2 ? x.z : x.w;
+}
+// A look at a barrier that never blocks, to be made ahead of the wait.
+MR_DEVICE bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
 }
 // Four rows (y) of 128 bytes at column x.
 MR_DEVICE void tma_gather4(void* dst, const CUtensorMap* map, int x, const int4& y,
@@ -208,6 +225,10 @@ MR_DEVICE void mm_arrive(uint64_t* bar, uint32_t to, uint32_t rank) {
 __device__ __noinline__ void wait_called(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                          unsigned* error) {
   wait_bounded(bar, parity, abort_flag, error);
+}
+MR_DEVICE void wait_mbar(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                         unsigned* error, bool seen) {
+  if (__builtin_expect(!seen, 0)) wait_called(bar, parity, abort_flag, error);
 }
 MR_DEVICE void wait_mbar(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                          unsigned* error) {
@@ -432,7 +453,8 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   if (tid == 0) {
     for (int s = 0; s < nst; ++s) {
       mbar_init(lfull + s, 1);
-      mbar_init(full + s, CG == 1 ? 5 : 8);  // four warps' exponents a CTA (CG = 1: the copies)
+      // four warps' exponents a CTA; the copies (CG = 2: the other CTA's)
+      mbar_init(full + s, 4 * CG + 1);
       mbar_init(empty + s, 1);
     }
     for (int s = 0; s < kMmRaw; ++s) {
@@ -444,7 +466,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       mbar_init(dempty + b, 4 * CG);
     }
     mbar_init(drain, 1);
-    mbar_init(done, 8);
+    mbar_init(done, rank == 0 ? 8 : 9);
     mbar_init(bye, 1);
     flags[0] = 0;
     fence_mbar_init();
@@ -537,7 +559,22 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    if (rank != 0 || !elect_one()) return;
+    if (!elect_one()) return;
+    if (rank != 0) {
+      // this CTA's copies have landed: tell the leader
+      uint32_t slot = 0, phase = 0;
+      for (int item = first; item < n_items; item += stride)
+        for (int st = 0; st < p.nstages; ++st) {
+          wait_mbar(lfull + slot, phase, flags, p.error);
+          mm_arrive<CG>(full + slot, 0, rank);
+          if (++slot == (uint32_t)nst) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+      mbar_arrive(done);
+      return;
+    }
     const int sfc = mm_sf_cols(p.ntile), sfw = mm_sf_word(p.ntile);
     const uint32_t a0 = smem_u32(smem), b0 = smem_u32(bring);
     uint32_t slot = 0, phase = 0, t = 0;
@@ -551,6 +588,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         const uint32_t sfa = 2 * p.ntile + slot * sfc, sfb = sfa + 16;
         const uint32_t at = a0 + slot * 2 * kMmAPiece, bt = b0 + slot * 2 * b_piece;
         wait_mbar(full + slot, phase, flags, p.error);
+        if constexpr (CG == 2) wait_mbar(lfull + slot, phase, flags, p.error);
         tc_fence_after();
         // a row's last stage may hold fewer than eight steps of 64
         const int steps = min(8, (p.groups - st * 16 + 1) / 2);
@@ -585,61 +623,51 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     const int sfc = mm_sf_cols(p.ntile), sfw = mm_sf_word(p.ntile);
     const int slot_rows = mm_raw_rows(p.ntile);
     uint32_t slot = 0, phase = 0, rslot = 0, rphase = 0;
-    struct Stage {
-      uint4 a[4], b[kMmB];  // rows lane + 32 i
-    };
-    int64_t left =
-        first < n_items ? (int64_t)((n_items - 1 - first) / stride + 1) * p.nstages : 0;
-    auto fetch = [&](Stage& v) {
-      if (left-- <= 0) return;
-      wait_mbar(rfull + rslot, rphase, flags, p.error);
-      const uint4* src = raw + rslot * slot_rows + lane;
+    for (int item = first; item < n_items; item += stride)
+      for (int st = 0; st < p.nstages; ++st) {
+        wait_mbar(rfull + rslot, rphase, flags, p.error);
+        const bool free = mbar_test(empty + slot, phase ^ 1u);
+        const uint4* src = raw + rslot * slot_rows + lane;
+        uint4 a[4], b[kMmB];  // rows lane + 32 i
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v.a[i] = src[32 * i];
+        for (int i = 0; i < 4; ++i) a[i] = src[32 * i];
 #pragma unroll
-      for (int i = 0; i < kMmB; ++i)
-        v.b[i] = 32 * i < p.ntile ? src[kMmRows + 32 * i] : make_uint4(0, 0, 0, 0);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(rempty + rslot);
-      if (++rslot == kMmRaw) {
-        rslot = 0;
-        rphase ^= 1u;
-      }
-    };
-    auto hand_on = [&](const Stage& v) {
-      wait_mbar(empty + slot, phase ^ 1u, flags, p.error);
-      tc_fence_after();
-      const uint32_t t = lane_t + slot * sfc;
+        for (int i = 0; i < kMmB; ++i)
+          b[i] = 32 * i < p.ntile ? src[kMmRows + 32 * i] : make_uint4(0, 0, 0, 0);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(rempty + rslot);
+        if (++rslot == kMmRaw) {
+          rslot = 0;
+          rphase ^= 1u;
+        }
+        wait_mbar(empty + slot, phase ^ 1u, flags, p.error, free);
+        tc_fence_after();
+        // columns 4 w + i (B: sfw w + i): word w of rows lane + 32 i
+        const uint32_t t = lane_t + slot * sfc;
+        uint32_t x[16];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        auto word = [&](const uint4& x) { return w == 0 ? x.x : w == 1 ? x.y : w == 2 ? x.z : x.w; };
-        tmem_st4(t + 4 * w, word(v.a[0]), word(v.a[1]), word(v.a[2]), word(v.a[3]));
-        const uint32_t tb = t + 16 + w * sfw;
-        tmem_st4(tb, word(v.b[0]), word(v.b[1]), word(v.b[2]), word(v.b[3]));
-        if (p.ntile > 128) tmem_st4(tb + 4, word(v.b[4]), word(v.b[5]), 0, 0);
+        for (int k = 0; k < 16; ++k) x[k] = word_of(a[k & 3], k >> 2);
+        tmem_st16(t, x);
+        if (p.ntile > 128) {
+          uint32_t y[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            y[k] = (k & 7) < kMmB ? word_of(b[(k & 7) < kMmB ? k & 7 : 0], k >> 3) : 0u;
+          tmem_st32(t + 16, y);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) x[k] = word_of(b[k & 3], k >> 2);
+          tmem_st16(t + 16, x);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mm_arrive<CG>(full + slot, 0, rank);
+        if (++slot == (uint32_t)nst) {
+          slot = 0;
+          phase ^= 1u;
+        }
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      // one warp vouches for the CTA's copies too
-      if (CG == 2 && warp == 8) wait_mbar(lfull + slot, phase, flags, p.error);
-      if (lane == 0) mm_arrive<CG>(full + slot, 0, rank);
-      if (++slot == (uint32_t)nst) {
-        slot = 0;
-        phase ^= 1u;
-      }
-    };
-    Stage v0, v1;  // the next stage is on its way while one is stored
-    int64_t todo = left;
-    fetch(v0);
-    for (; todo > 0; todo -= 2) {
-      fetch(v1);
-      hand_on(v0);
-      if (todo > 1) {
-        fetch(v0);
-        hand_on(v1);
-      }
-    }
     if (lane == 0) mbar_arrive(done);
   } else if (warp >= 12) {
     // -------------------------------------------------------------- gathers

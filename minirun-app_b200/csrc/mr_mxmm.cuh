@@ -576,17 +576,18 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       return;
     }
     const int sfc = mm_sf_cols(p.ntile), sfw = mm_sf_word(p.ntile);
-    const uint32_t a0 = smem_u32(smem), b0 = smem_u32(bring);
+    const uint64_t ad0 = umma_desc_sw128(smem_u32(smem)), bd0 = umma_desc_sw128(smem_u32(bring));
     uint32_t slot = 0, phase = 0, t = 0;
     for (int item = first; item < n_items; item += stride, ++t) {
       it.at(item);
       const uint32_t db = t & 1u;
       const int nn = mm_round(it.n);
+      const uint32_t id0 = umma_idesc_mxf4<CG>(nn, 0), id1 = umma_idesc_mxf4<CG>(nn, 1);
       wait_mbar(dempty + db, ((t >> 1) & 1u) ^ 1u, flags, p.error);
       const uint32_t d_t = db * p.ntile;
       for (int st = 0; st < p.nstages; ++st) {
         const uint32_t sfa = 2 * p.ntile + slot * sfc, sfb = sfa + 16;
-        const uint32_t at = a0 + slot * 2 * kMmAPiece, bt = b0 + slot * 2 * b_piece;
+        const uint64_t ad = ad0 + slot * (2 * kMmAPiece >> 4), bd = bd0 + slot * (2 * b_piece >> 4);
         wait_mbar(full + slot, phase, flags, p.error);
         if constexpr (CG == 2) wait_mbar(lfull + slot, phase, flags, p.error);
         tc_fence_after();
@@ -595,10 +596,9 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
           if (kk < steps)
-            tc_mma_mxf4<CG>(d_t, umma_desc_sw128(at + (kk >> 2) * kMmAPiece + (kk & 3) * 32),
-                            umma_desc_sw128(bt + (kk >> 2) * b_piece + (kk & 3) * 32),
-                            umma_idesc_mxf4<CG>(nn, kk & 1), sfa + 4 * (kk >> 1),
-                            sfb + sfw * (kk >> 1), (st | kk) ? 1u : 0u);
+            tc_mma_mxf4<CG>(d_t, ad + ((kk >> 2) * (kMmAPiece >> 4) + (kk & 3) * 2),
+                            bd + ((kk >> 2) * (b_piece >> 4) + (kk & 3) * 2), (kk & 1) ? id1 : id0,
+                            sfa + 4 * (kk >> 1), sfb + sfw * (kk >> 1), (st | kk) ? 1u : 0u);
         mm_commit<CG>(empty + slot);
         if (++slot == (uint32_t)nst) {
           slot = 0;

@@ -81,7 +81,9 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
   p.arows = a->out_features;
   p.out_features = w->out_features;
   p.E = plan ? w->experts : 1;
-  p.top_k = plan ? plan->top_k : 1;
+  const uint64_t k = plan ? plan->top_k : 1;
+  while ((1ull << p.k_shift) < k) ++p.k_shift;
+  p.k_mul = (uint32_t)(((1ull << (31 + p.k_shift)) + k - 1) / k);
   p.groups = (int)(w->in_features / 32);
   p.nstages = (int)((w->in_features + kMmK - 1) / kMmK);
   p.out_f32 = out_dtype == MR_DTYPE_F32;

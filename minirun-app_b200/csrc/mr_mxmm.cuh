@@ -54,7 +54,7 @@ constexpr int kMmMaxN = 176;     // activation rows of a tile: two accumulators 
                                  // slots of exponents fit the 512 TMEM columns
 constexpr int kMmB = (kMmMaxN + 31) / 32;
 constexpr int kMmThreads = 384;  // plus the gather warps
-constexpr int kMmGatherWarps = 4;
+constexpr int kMmGatherWarps = 4;  // sixteen warps in all: more would leave 96 registers each
 constexpr int kMmAPiece = kMmRows * 128;
 constexpr int kMmRaw = 3;  // slots of the exponents' ring in shared memory
 
@@ -74,7 +74,8 @@ struct MmParams {
   void* out;                // [rows, out]
   unsigned* error;
   int64_t rows, arows, out_features;
-  int E, top_k;
+  int E;
+  uint32_t k_mul, k_shift;  // pair / top_k, see mm_act_row
   int groups;           // in / 32
   int nstages, mtiles;
   int ntile, box, nst;  // tile width, rows of an activation box, ring stages
@@ -240,12 +241,14 @@ MR_DEVICE void wait_mbar(uint64_t* bar, uint32_t parity, volatile int* abort_fla
 // An expert's n rows in tiles of equal width: as few as ntile allows, none
 // empty.
 MR_DEVICE int mm_width(int n, int ntile) {
-  const int c = (n + ntile - 1) / ntile;
-  return c > 0 ? mm_round((n + c - 1) / c) : 16;
+  if (n <= ntile) return max(mm_round(n), 16);
+  const uint32_t c = (uint32_t)(n + ntile - 1) / (uint32_t)ntile;
+  return mm_round((int)((uint32_t)(n + c - 1) / c));
 }
 MR_DEVICE int mm_tiles(int n, int ntile) {
-  const int w = mm_width(n, ntile);
-  return (n + w - 1) / w;
+  if (n <= ntile) return n > 0;
+  const uint32_t w = mm_width(n, ntile);
+  return (int)((uint32_t)(n + w - 1) / w);
 }
 
 // Walks the CTA's (or pair's) tiles in order: item -> expert, rows, and the
@@ -254,13 +257,23 @@ template <int CG>
 struct MmWalk {
   const int* goff;   // [E + 1] first row of each expert
   const int* gtile;  // [E + 1] first row tile of each expert
-  int mtiles, ntile;
+  int E, mtiles, ntile;
   int m_in;          // the CTA's first row in a tile
-  int e = 0, row0 = 0, n = 0, m0 = 0;
+  int e;             // the first tile's expert, then the last one's
+  int row0, n, m0;
   MR_DEVICE void at(int item) {
-    const int t = item / mtiles;
+    const int t = (int)((uint32_t)item / (uint32_t)mtiles);
     m0 = (item - t * mtiles) * (kMmRows * CG) + m_in;
-    while (gtile[e + 1] <= t) ++e;
+    if (gtile[e + 1] <= t) {
+      int hi = E;  // gtile[e] <= t < gtile[hi]
+      while (hi - e > 1) {
+        const int mid = (e + hi) >> 1;
+        if (gtile[mid] <= t)
+          e = mid;
+        else
+          hi = mid;
+      }
+    }
     const int all = goff[e + 1] - goff[e];
     const int w = mm_width(all, ntile);
     const int first = (t - gtile[e]) * w;
@@ -274,8 +287,10 @@ struct MmWalk {
 // The token row that sorted row r takes its activations from.
 MR_DEVICE int64_t mm_act_row(const MmParams& p, int64_t r) {
   if (p.order) {
-    const int pair = __ldg(p.order + r);
-    r = pair < 0 ? 0 : pair / p.top_k;
+    // pair / top_k for pair < 2^31: k_mul = ceil(2^(31 + k_shift) / top_k) with
+    // 2^k_shift >= top_k
+    const int pair = max(__ldg(p.order + r), 0);
+    r = (int64_t)(((uint64_t)(uint32_t)pair * p.k_mul) >> (31 + p.k_shift));
   }
   return min(r, p.arows - 1);
 }
@@ -441,8 +456,8 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   uint64_t* bye = done + 1;           // the other CTA needs this one's memory no more
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bye + 1);
   volatile int* flags = reinterpret_cast<volatile int*>(tslot + 1);
-  int* scan = reinterpret_cast<int*>(tslot + 2);  // [16] warp sums
-  int* goff = scan + 16;
+  int* scan = reinterpret_cast<int*>(tslot + 2);  // [18] warp sums, [31] first tile's expert
+  int* goff = scan + 32;
   int* gtile = goff + p.E + 1;
   // CG = 1: the copies complete on `full` itself
   uint64_t* cfull = CG == 1 ? full : lfull;
@@ -473,44 +488,51 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   }
   if (warp == 4) mm_tmem_alloc<CG>(tslot);
   pdl_wait_and_release();
-  // the group table: thread i has experts 4i .. 4i+3 (E <= 1024: the first 256 threads)
-  {
-    int cnt[4], sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = 4 * tid + i;
-      cnt[i] = 0;
-      if (e < p.E) {
-        int a = 0, b = (int)p.rows;
-        if (p.offsets) {
-          a = min(max(__ldg(p.offsets + e), 0), (int)p.rows);
-          b = min(max(__ldg(p.offsets + e + 1), a), (int)p.rows);
-        }
-        goff[e] = a;
-        if (e + 1 == p.E) goff[p.E] = b;
-        cnt[i] = mm_tiles(b - a, p.ntile);
+  // The group table. The threads have an expert each (of which there may be
+  // several rounds); the one with this CTA's first tile says so.
+  if (tid == 0) {
+    goff[p.E] = 0;
+    gtile[p.E] = 0;
+    scan[31] = 0;
+  }
+  const int tile0 = (int)((uint32_t)first / (uint32_t)p.mtiles);
+  for (int base = 0; base < p.E; base += kMmThreads) {
+    const int e = base + tid;
+    int a = 0, b = (int)p.rows, cnt = 0;
+    if (e < p.E && tid < kMmThreads) {
+      if (p.offsets) {
+        a = min(max(__ldg(p.offsets + e), 0), (int)p.rows);
+        b = min(max(__ldg(p.offsets + e + 1), a), (int)p.rows);
       }
-      sum += cnt[i];
+      goff[e] = a;
+      cnt = mm_tiles(b - a, p.ntile);
     }
-    int incl = sum;
+    int run = 0;
+    if (p.E > 1) {
+      int incl = cnt;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int n = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += n;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += n;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      // warps before this one, and the rounds before (at the end of the table)
+      int w = lane < warp ? scan[lane] : 0;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) w += __shfl_xor_sync(0xffffffffu, w, d);
+      run = gtile[p.E] + w + incl - cnt;
+      __syncthreads();
     }
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    int run = incl - sum;
-    for (int w = 0; w < warp; ++w) run += scan[w];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = 4 * tid + i;
-      if (e < p.E) {
-        gtile[e] = run;
-        run += cnt[i];
-        if (e + 1 == p.E) gtile[p.E] = run;
+    if (e < p.E && tid < kMmThreads) {
+      gtile[e] = run;
+      if (cnt > 0 && tile0 >= run && tile0 < run + cnt) scan[31] = e;
+      if (e + 1 == p.E || tid + 1 == kMmThreads) {
+        goff[p.E] = b;
+        gtile[p.E] = run + cnt;
       }
     }
+    if (base + kMmThreads < p.E) __syncthreads();
   }
   tc_fence_before();
   if constexpr (CG == 1)
@@ -520,7 +542,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   tc_fence_after();
   constexpr uint32_t tbase = 0;  // all 512 columns are this CTA's: they start at 0
   const int n_items = gtile[p.E] * p.mtiles;
-  MmWalk<CG> it{goff, gtile, p.mtiles, p.ntile, (int)rank * kMmRows};
+  MmWalk<CG> it{goff, gtile, p.E, p.mtiles, p.ntile, (int)rank * kMmRows, scan[31], 0, 0, 0};
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -681,6 +703,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       int4 rows[kMine];  // every kMmGatherWarps-th gather is this warp's
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
+        if (w + i * kMmGatherWarps >= nq) break;
         const int r0 = it.row0 + (int)rank * half + 4 * (w + i * kMmGatherWarps);
         const int r1 = it.row0 + it.n - 1;  // rows past the tile's end repeat its last
         rows[i] =
@@ -741,10 +764,13 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     if (warp == 4) {
       wait_mbar(done, 0, flags, p.error);
       wait_mbar(drain, 0, flags, p.error);
-      // the last arrivals at the ring's barriers, which nobody else waits for
-      const int64_t stages = (int64_t)t * p.nstages;
-      for (int s = 0; s < nst && s < stages; ++s)
-        wait_mbar(empty + s, (uint32_t)((stages - 1 - s) / nst) & 1u, flags, p.error);
+      if (CG == 2 && t > 0) {
+        // the last arrivals at the ring's barriers, which nobody else waits for:
+        // use j of the ring is slot j % nst, phase j / nst
+        const uint32_t last = t * (uint32_t)p.nstages - 1, a = last / nst, r = last - a * nst;
+        for (int s = 0; s < nst && (uint32_t)s <= last; ++s)
+          wait_mbar(empty + s, ((uint32_t)s <= r ? a : a - 1) & 1u, flags, p.error);
+      }
       tc_fence_after();
       mm_tmem_dealloc<CG>();
       if constexpr (CG == 2) {

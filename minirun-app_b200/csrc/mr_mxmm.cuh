@@ -236,6 +236,23 @@ MR_DEVICE void wait_mbar(uint64_t* bar, uint32_t parity, volatile int* abort_fla
   if (__builtin_expect(!mbar_try_wait(bar, parity), 0)) wait_called(bar, parity, abort_flag, error);
 }
 
+MR_DEVICE void put(float* p, float v) { *p = v; }
+MR_DEVICE void put(uint16_t* p, float v) { *p = f32_to_bf16_bits(v); }
+// One result of each of 16 rows (`left` of which exist), `pitch` apart. The
+// whole chunk has no branch between its stores: with one for each row the
+// epilogue took 36 cycles a row, longer than the MMAs of a narrow matrix.
+template <typename T>
+MR_DEVICE void store16(T* p, int64_t pitch, int left, const float (&v)[16]) {
+  if (left >= 16) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) put(p + i * pitch, v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < left) put(p + i * pitch, v[i]);
+  }
+}
+
 // ------------------------------------------------------------------- tiles
 
 // An expert's n rows in tiles of equal width: as few as ntile allows, none
@@ -742,17 +759,12 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       for (int c = 0; c < it.n; c += 16) {
         float v[16];
         tmem_ld16(d_t + c, v);
-        if (o < p.out_features) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (c + i >= it.n) break;
-            const int64_t at = ((int64_t)it.row0 + c + i) * p.out_features + o;
-            if (p.out_f32)
-              reinterpret_cast<float*>(p.out)[at] = v[i];
-            else
-              reinterpret_cast<uint16_t*>(p.out)[at] = f32_to_bf16_bits(v[i]);
-          }
-        }
+        if (o >= p.out_features) continue;
+        const int64_t at = ((int64_t)it.row0 + c) * p.out_features + o;
+        if (p.out_f32)
+          store16(reinterpret_cast<float*>(p.out) + at, p.out_features, it.n - c, v);
+        else
+          store16(reinterpret_cast<uint16_t*>(p.out) + at, p.out_features, it.n - c, v);
       }
       tc_fence_before();
       __syncwarp();

@@ -274,6 +274,7 @@ struct mr_ctx {
   size_t fixed_bytes = 0;
   unsigned* d_error = nullptr;
   unsigned* d_counters = nullptr;  // kMaxCounters
+  unsigned kernel_attrs = 0;  // kernels whose attributes are set on this device, a bit each
   int kernel_path = 0;  // 0 auto, 1 register-streaming GEMV, 2 TMA-pipelined GEMV
   // encoded TMA tensor maps (128-byte CUtensorMap each), keyed by
   // (base, rows, width, box rows, kind)

@@ -27,6 +27,19 @@ inline cudaError_t set_device(const mr_ctx* ctx) {
   return e == cudaSuccess && cur != ctx->device ? cudaSetDevice(ctx->device) : e;
 }
 
+// Sets a kernel's attributes the first time a context launches it.
+enum KernelAttr : unsigned {
+  kAttrSort = 1u,
+  kAttrProduct = 2u  // and the next three bits: mxmm_kernel's instances
+};
+template <typename F>
+inline cudaError_t attrs_once(mr_ctx* ctx, unsigned bit, F&& set) {
+  if (ctx->kernel_attrs & bit) return cudaSuccess;
+  const cudaError_t e = set();
+  if (e == cudaSuccess) ctx->kernel_attrs |= bit;
+  return e;
+}
+
 // The shape and pointers of sorted tokens (mr_sort.cu).
 mr_status check_plan(mr_ctx* ctx, const mr_sorted* s);
 

@@ -117,7 +117,9 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
                          : (wide ? mxmm_kernel<true, 2> : mxmm_kernel<false, 2>);
   cudaError_t e = set_device(ctx);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmSmem);
+    e = attrs_once(ctx, kAttrProduct << (2 * (cg - 1) + wide), [&] {
+      return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmSmem);
+    });
   if (e == cudaSuccess) {
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

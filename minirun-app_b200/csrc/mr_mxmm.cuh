@@ -56,6 +56,7 @@ constexpr int kMmB = (kMmMaxN + 31) / 32;
 constexpr int kMmThreads = 384;  // plus the gather warps
 constexpr int kMmGatherWarps = 4;  // sixteen warps in all: more would leave 96 registers each
 constexpr int kMmAPiece = kMmRows * 128;
+constexpr int kMmTokens = kMmThreads;  // rows whose tokens are looked up at the start
 constexpr int kMmRaw = 3;  // slots of the exponents' ring in shared memory
 
 // The MMAs' N, and a tile's width, step by 16.
@@ -88,7 +89,7 @@ struct MmMaps {
 // Shared memory: ring of codes, ring of exponents, barriers, group table.
 inline int mm_stage_bytes(int ntile, int cg) { return 2 * (kMmAPiece + ntile / cg * 128); }
 inline int mm_fixed_bytes(int E, int ntile) {
-  return 1024 + kMmRaw * mm_raw_rows(ntile) * 16 + 768 + 2 * (E + 1) * 4;
+  return 1024 + kMmRaw * mm_raw_rows(ntile) * 16 + 768 + 2 * (E + 1) * 4 + kMmTokens * 4;
 }
 
 // ------------------------------------------------------------ instructions
@@ -301,15 +302,17 @@ struct MmWalk {
 
 // ------------------------------------------------------------ exponents
 
-// The token row that sorted row r takes its activations from.
-MR_DEVICE int64_t mm_act_row(const MmParams& p, int64_t r) {
-  if (p.order) {
-    // pair / top_k for pair < 2^31: k_mul = ceil(2^(31 + k_shift) / top_k) with
-    // 2^k_shift >= top_k
-    const int pair = max(__ldg(p.order + r), 0);
-    r = (int64_t)(((uint64_t)(uint32_t)pair * p.k_mul) >> (31 + p.k_shift));
-  }
-  return min(r, p.arows - 1);
+// The row of `a` that a pair takes its activations from. pair / top_k for pair
+// < 2^31: k_mul = ceil(2^(31 + k_shift) / top_k) with 2^k_shift >= top_k.
+MR_DEVICE int64_t mm_pair_row(const MmParams& p, int pair) {
+  const uint64_t t = ((uint64_t)(uint32_t)max(pair, 0) * p.k_mul) >> (31 + p.k_shift);
+  return min((int64_t)t, p.arows - 1);
+}
+// The same of sorted row r. Few rows have their tokens in shared memory.
+MR_DEVICE int64_t mm_act_row(const MmParams& p, const int* tok, int64_t r) {
+  if (!p.order) return min(r, p.arows - 1);
+  if (p.rows <= kMmTokens) return tok[r];
+  return mm_pair_row(p, __ldg(p.order + r));
 }
 
 // 16 bytes at an aligned address, of which only [lo, hi) may be read.
@@ -380,7 +383,7 @@ struct MmScaleRegs {
 template <int NB, bool WIDE, bool IS_A, int CG>
 MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lane, int first,
                               int stride, int n_items, uint4* raw, uint64_t* rfull,
-                              uint64_t* rempty, volatile int* flags) {
+                              uint64_t* rempty, const int* tok, volatile int* flags) {
   const int slot_rows = mm_raw_rows(p.ntile);
   const uint8_t* lo = IS_A ? p.w_scales : p.a_scales;
   const uint8_t* hi = lo + (IS_A ? (int64_t)p.E * p.out_features : p.arows) * p.groups;
@@ -396,7 +399,7 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lan
       const int r = min(lane + 32 * i, have - 1);
       const int64_t row =
           IS_A ? (int64_t)it.e * p.out_features + min((int64_t)it.m0 + r, p.out_features - 1)
-               : mm_act_row(p, (int64_t)it.row0 + r);
+               : mm_act_row(p, tok, (int64_t)it.row0 + r);
       src[i] = 32 * i < have ? lo + row * p.groups : nullptr;
     }
   };
@@ -476,17 +479,17 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   int* scan = reinterpret_cast<int*>(tslot + 2);  // [18] warp sums, [31] first tile's expert
   int* goff = scan + 32;
   int* gtile = goff + p.E + 1;
-  // CG = 1: the copies complete on `full` itself
-  uint64_t* cfull = CG == 1 ? full : lfull;
-
+  int* tok = gtile + p.E + 1;  // [kMmTokens]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = CG == 1 ? 0 : cluster_rank();
   const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+  // the leader's copies complete on `full` itself, the other CTA's on a
+  // barrier of its own, whose arrival is passed on
+  uint64_t* cfull = rank == 0 ? full : lfull;
   if (tid == 0) {
     for (int s = 0; s < nst; ++s) {
       mbar_init(lfull + s, 1);
-      // four warps' exponents a CTA; the copies (CG = 2: the other CTA's)
-      mbar_init(full + s, 4 * CG + 1);
+      mbar_init(full + s, 5 * CG);  // a CTA's copies and four warps' exponents
       mbar_init(empty + s, 1);
     }
     for (int s = 0; s < kMmRaw; ++s) {
@@ -513,6 +516,8 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     scan[31] = 0;
   }
   const int tile0 = (int)((uint32_t)first / (uint32_t)p.mtiles);
+  if (p.order && p.rows <= kMmTokens && tid < p.rows)
+    tok[tid] = (int)mm_pair_row(p, __ldg(p.order + tid));
   for (int base = 0; base < p.E; base += kMmThreads) {
     const int e = base + tid;
     int a = 0, b = (int)p.rows, cnt = 0;
@@ -628,16 +633,20 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         const uint32_t sfa = 2 * p.ntile + slot * sfc, sfb = sfa + 16;
         const uint64_t ad = ad0 + slot * (2 * kMmAPiece >> 4), bd = bd0 + slot * (2 * b_piece >> 4);
         wait_mbar(full + slot, phase, flags, p.error);
-        if constexpr (CG == 2) wait_mbar(lfull + slot, phase, flags, p.error);
         tc_fence_after();
         // a row's last stage may hold fewer than eight steps of 64
         const int steps = min(8, (p.groups - st * 16 + 1) / 2);
+        auto mma = [&](int kk) {
+          tc_mma_mxf4<CG>(d_t, ad + ((kk >> 2) * (kMmAPiece >> 4) + (kk & 3) * 2),
+                          bd + ((kk >> 2) * (b_piece >> 4) + (kk & 3) * 2), (kk & 1) ? id1 : id0,
+                          sfa + 4 * (kk >> 1), sfb + sfw * (kk >> 1), (st | kk) ? 1u : 0u);
+        };
+        if (steps == 8) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          if (kk < steps)
-            tc_mma_mxf4<CG>(d_t, ad + ((kk >> 2) * (kMmAPiece >> 4) + (kk & 3) * 2),
-                            bd + ((kk >> 2) * (b_piece >> 4) + (kk & 3) * 2), (kk & 1) ? id1 : id0,
-                            sfa + 4 * (kk >> 1), sfb + sfw * (kk >> 1), (st | kk) ? 1u : 0u);
+          for (int kk = 0; kk < 8; ++kk) mma(kk);
+        } else {
+          for (int kk = 0; kk < steps; ++kk) mma(kk);
+        }
         mm_commit<CG>(empty + slot);
         if (++slot == (uint32_t)nst) {
           slot = 0;
@@ -652,10 +661,10 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     // ------------------------------------------- exponents to shared memory
     if (warp == 2)
       mm_load_scales<4, WIDE, true>(p, it, lane, first, stride, n_items, raw, rfull, rempty,
-                                    flags);
+                                    tok, flags);
     else
       mm_load_scales<kMmB, WIDE, false>(p, it, lane, first, stride, n_items, raw, rfull,
-                                                rempty, flags);
+                                                rempty, tok, flags);
   } else if (warp >= 8 && warp < 12) {
     // -------------------------------------------- exponents to tensor memory
     const uint32_t lane_t = tbase + ((uint32_t)((warp & 3) * 32) << 16) + 2 * p.ntile;
@@ -724,8 +733,8 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         const int r0 = it.row0 + (int)rank * half + 4 * (w + i * kMmGatherWarps);
         const int r1 = it.row0 + it.n - 1;  // rows past the tile's end repeat its last
         rows[i] =
-            make_int4((int)mm_act_row(p, min(r0, r1)), (int)mm_act_row(p, min(r0 + 1, r1)),
-                      (int)mm_act_row(p, min(r0 + 2, r1)), (int)mm_act_row(p, min(r0 + 3, r1)));
+            make_int4((int)mm_act_row(p, tok, min(r0, r1)), (int)mm_act_row(p, tok, min(r0 + 1, r1)),
+                      (int)mm_act_row(p, tok, min(r0 + 2, r1)), (int)mm_act_row(p, tok, min(r0 + 3, r1)));
       }
       for (int st = 0; st < p.nstages; ++st) {
         const int pieces = min(2, (p.groups - st * 16 + 7) / 8);

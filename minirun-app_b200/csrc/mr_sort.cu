@@ -42,6 +42,7 @@ struct SortParams {
 constexpr int kSortThreads = 1024;
 constexpr int kSortCluster = 16;  // CTAs of a large sort's cluster
 constexpr int64_t kSortOneCta = 4096;  // pairs one CTA sorts alone
+constexpr int kSortSmem = 4 * (kSortThreads / 32 * kMaxExperts + 2 * kMaxExperts + 32);
 constexpr int kSortBatch = 4;          // groups of 32 pairs a warp has in registers
 constexpr int kSortColumn = 8;         // histogram entries loaded together
 
@@ -685,10 +686,14 @@ mr_status mr_moe_sort(mr_ctx* ctx, const int32_t* ids, int64_t tokens, int32_t t
     p.chunk = (per + 31) / 32 * 32;
     const size_t smem = sizeof(int) * ((size_t)warps * experts + 2 * experts + 32);
     cudaError_t e = set_device(ctx);
-    if (e == cudaSuccess && smem > 48 * 1024)
-      e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess && ctas > 8)
-      e = cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+      e = attrs_once(ctx, kAttrSort, [] {
+        const cudaError_t a = cudaFuncSetAttribute(
+            sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSmem);
+        return a != cudaSuccess ? a
+                                : cudaFuncSetAttribute(
+                                      sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      });
     if (e == cudaSuccess) {
       cudaLaunchAttribute attr[2];
       attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

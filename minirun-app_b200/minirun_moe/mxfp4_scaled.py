@@ -24,16 +24,20 @@ _IN_DTYPES = {torch.bfloat16: L.MR_DTYPE_BF16, torch.float16: L.MR_DTYPE_F16,
 _OUT_DTYPES = {torch.bfloat16: L.MR_DTYPE_BF16, torch.float32: L.MR_DTYPE_F32}
 
 
-def _checked(name: str, x: torch.Tensor) -> torch.Tensor:
-    """Rows of x that the quantiser can read in place: the last axis contiguous, the others one
-    stride apart."""
-    if x.dim() not in (2, 3) or not x.is_cuda or x.dtype not in _IN_DTYPES:
+def _checked(name: str, x: torch.Tensor):
+    """(x, its shape, row stride) for rows that the quantiser reads in place: the last axis
+    contiguous, the rows one stride apart; otherwise of a copy."""
+    shape = x.shape
+    if len(shape) not in (2, 3) or not x.is_cuda or x.dtype not in _IN_DTYPES:
         raise MXFP4BridgeError(
             f"{name} must be a CUDA bfloat16, float16 or float32 [rows, inFeatures] or [experts, "
-            f"rows, inFeatures] tensor, got {list(x.shape)} {x.dtype} on {x.device}")
-    if x.dim() == 2 and x.stride(1) == 1 and (x.shape[0] <= 1 or x.stride(0) >= x.shape[1]):
-        return x
-    return x if x.is_contiguous() else x.contiguous()
+            f"rows, inFeatures] tensor, got {list(shape)} {x.dtype} on {x.device}")
+    n = shape[-1]
+    if x.is_contiguous():
+        return x, shape, n
+    if len(shape) == 2 and x.stride(1) == 1 and (shape[0] <= 1 or x.stride(0) >= n):
+        return x, shape, max(x.stride(0), n)
+    return x.contiguous(), shape, n
 
 
 def _weights_of(packed: torch.Tensor, scales: torch.Tensor, rows: int, width: int,
@@ -49,46 +53,47 @@ def mxfp4_quantize(x: torch.Tensor, values: bool = False):
     """``x`` [rows, in] or [experts, rows, in] in MXFP4 (see mr_mxfp4_quantize for the rounding).
     With ``values`` the pair (codes, values): the numbers the codes stand for in x's type, what a
     training step with 4-bit forward values multiplies with."""
-    x = _checked("x", x)
-    shape = x.shape
-    width = shape[-1]
-    rows = shape[0] if x.dim() == 2 else shape[0] * shape[1]
+    x, shape, stride = _checked("x", x)
+    if len(shape) == 2:
+        experts, (rows, width) = None, shape
+        lead = (rows,)
+    else:
+        experts, rows, width = shape
+        lead = (experts, rows)
     if width % 32 != 0 or width == 0:
         raise MXFP4BridgeError(
             f"inFeatures {width} is not a multiple of groupSize 32; partial final groups are "
             "not supported")
     dev = x.device
-    packed = x.new_empty(shape[:-1] + (width // 8,), dtype=torch.int32)
-    scales = x.new_empty(shape[:-1] + (width // 32,), dtype=torch.uint8)
+    packed = x.new_empty((*lead, width // 8), dtype=torch.int32)
+    scales = x.new_empty((*lead, width // 32), dtype=torch.uint8)
     out = x.new_empty(shape) if values else None
     ctx = Context.get(dev.index)
-    stride = max(x.stride(0), width) if x.dim() == 2 else width
     st = L.load().mr_mxfp4_quantize(
-        ctx.handle, x.data_ptr(), _IN_DTYPES[x.dtype], rows, width, stride, packed.data_ptr(),
-        scales.data_ptr(), None if out is None else out.data_ptr(), _raw_stream(dev))
+        ctx.handle, x.data_ptr(), _IN_DTYPES[x.dtype], rows if experts is None else rows * experts,
+        width, stride, packed.data_ptr(), scales.data_ptr(),
+        None if out is None else out.data_ptr(), _raw_stream(dev))
     if st:
         ctx.check("mr_mxfp4_quantize", st)
-    experts = shape[0] if x.dim() == 3 else None
-    q = _weights_of(packed, scales, shape[-2], width, experts)
+    q = _weights_of(packed, scales, rows, width, experts)
     return (q, out) if values else q
 
 
 def mxfp4_quantize_swiglu(gate_up: torch.Tensor, limit: float = 0.0) -> MXFP4Weights:
     """``silu(gate) * up`` of rows ``[gate | up]`` in MXFP4, [rows, in]; ``limit`` > 0 clamps
     ``gate <= limit`` and ``-limit <= up <= limit`` first."""
-    x = _checked("gate_up", gate_up)
-    if x.dim() != 2 or x.shape[1] % 64 != 0 or x.shape[1] == 0:
+    x, shape, stride = _checked("gate_up", gate_up)
+    if len(shape) != 2 or shape[1] % 64 != 0 or shape[1] == 0:
         raise MXFP4BridgeError(
-            f"gate_up must be [rows, 2 * inter] with inter a multiple of 32, got {list(x.shape)}")
-    rows, width = x.shape[0], x.shape[1] // 2
+            f"gate_up must be [rows, 2 * inter] with inter a multiple of 32, got {list(shape)}")
+    rows, width = shape[0], shape[1] // 2
     dev = x.device
     packed = x.new_empty((rows, width // 8), dtype=torch.int32)
     scales = x.new_empty((rows, width // 32), dtype=torch.uint8)
     ctx = Context.get(dev.index)
     st = L.load().mr_mxfp4_quantize_swiglu(
-        ctx.handle, x.data_ptr(), _IN_DTYPES[x.dtype], rows, width,
-        max(x.stride(0), 2 * width), limit, packed.data_ptr(), scales.data_ptr(),
-        _raw_stream(dev))
+        ctx.handle, x.data_ptr(), _IN_DTYPES[x.dtype], rows, width, stride, limit,
+        packed.data_ptr(), scales.data_ptr(), _raw_stream(dev))
     if st:
         ctx.check("mr_mxfp4_quantize_swiglu", st)
     return _weights_of(packed, scales, rows, width, None)

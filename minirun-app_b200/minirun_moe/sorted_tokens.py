@@ -106,21 +106,22 @@ def moe_sort(ids: torch.Tensor, experts: int) -> SortedTokens:
     return s
 
 
-def _rows(name: str, t: torch.Tensor, rows: int, plan: SortedTokens) -> torch.Tensor:
-    """[rows, hidden] with contiguous rows, of a supported type, on the plan's device."""
-    if t.dim() != 2 or t.shape[0] != rows:
-        raise AffineBridgeError(f"{name} must be [{rows}, hidden], got {list(t.shape)}")
+def _rows(name: str, t: torch.Tensor, rows: int, plan: SortedTokens):
+    """(rows with a contiguous last axis, hidden, row stride) of a [rows, hidden] tensor of a
+    supported type on the plan's device."""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows:
+        raise AffineBridgeError(f"{name} must be [{rows}, hidden], got {list(shape)}")
     if t.dtype not in _ROW_DTYPES:
         raise AffineBridgeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
     if t.device != plan.device:
         raise AffineBridgeError(f"{name} is on {t.device}, the sorted tokens on {plan.device}")
-    if t.stride(1) != 1 or (rows > 1 and t.stride(0) < t.shape[1]):
-        return t.contiguous()
-    return t
-
-
-def _stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
+    H = shape[1]
+    if t.is_contiguous():
+        return t, H, H
+    if t.stride(1) != 1 or (rows > 1 and t.stride(0) < H):
+        return t.contiguous(), H, H
+    return t, H, max(t.stride(0), H)
 
 
 def _weights(w: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
@@ -133,11 +134,10 @@ def _weights(w: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
 
 
 def _dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
-    x = _rows("x", x, plan.tokens, plan)
-    H = x.shape[1]
+    x, H, stride = _rows("x", x, plan.tokens, plan)
     xs = x.new_empty((plan.rows, H))
     ctx = Context.get(plan.device.index)
-    st = L.load().mr_moe_dispatch(ctx.handle, x.data_ptr(), _ROW_DTYPES[x.dtype], _stride(x), H,
+    st = L.load().mr_moe_dispatch(ctx.handle, x.data_ptr(), _ROW_DTYPES[x.dtype], stride, H,
                                   plan._ref, xs.data_ptr(), _raw_stream(plan.device))
     if st:
         ctx.check("mr_moe_dispatch", st)
@@ -146,12 +146,11 @@ def _dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
 
 def moe_dispatch_backward(dxs: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     """Gradient of ``moe_dispatch``: ``dx[t] = sum_j dxs[inverse[t, j]]``, fp32 sums."""
-    dxs = _rows("dxs", dxs, plan.rows, plan)
-    H = dxs.shape[1]
+    dxs, H, stride = _rows("dxs", dxs, plan.rows, plan)
     dx = dxs.new_empty((plan.tokens, H))
     ctx = Context.get(plan.device.index)
     st = L.load().mr_moe_dispatch_backward(ctx.handle, dxs.data_ptr(), _ROW_DTYPES[dxs.dtype],
-                                           _stride(dxs), H, plan._ref, dx.data_ptr(),
+                                           stride, H, plan._ref, dx.data_ptr(),
                                            _raw_stream(plan.device))
     if st:
         ctx.check("mr_moe_dispatch_backward", st)
@@ -159,20 +158,21 @@ def moe_dispatch_backward(dxs: torch.Tensor, plan: SortedTokens) -> torch.Tensor
 
 
 def _combine(ys, weights, plan, base) -> torch.Tensor:
-    ys = _rows("ys", ys, plan.rows, plan)
-    H = ys.shape[1]
+    ys, H, stride = _rows("ys", ys, plan.rows, plan)
     weights = _weights(weights, plan)
+    at = None
     if base is not None:
         if base.shape != (plan.tokens, H) or base.dtype != ys.dtype or base.device != ys.device:
             raise AffineBridgeError(
                 f"base must be [{plan.tokens}, {H}] {ys.dtype} on {ys.device}, got "
                 f"{list(base.shape)} {base.dtype} on {base.device}")
         base = base.contiguous()
+        at = base.data_ptr()
     out = ys.new_empty((plan.tokens, H))
     ctx = Context.get(plan.device.index)
-    st = L.load().mr_moe_combine(ctx.handle, ys.data_ptr(), _ROW_DTYPES[ys.dtype], _stride(ys), H,
-                                 weights.data_ptr(), None if base is None else base.data_ptr(),
-                                 plan._ref, out.data_ptr(), _raw_stream(plan.device))
+    st = L.load().mr_moe_combine(ctx.handle, ys.data_ptr(), _ROW_DTYPES[ys.dtype], stride, H,
+                                 weights.data_ptr(), at, plan._ref, out.data_ptr(),
+                                 _raw_stream(plan.device))
     if st:
         ctx.check("mr_moe_combine", st)
     return out
@@ -181,10 +181,9 @@ def _combine(ys, weights, plan, base) -> torch.Tensor:
 def moe_combine_backward(dout: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor,
                          plan: SortedTokens) -> tuple[torch.Tensor, torch.Tensor]:
     """Gradients ``(dys, dweights)`` of ``moe_combine``; that of ``base`` is ``dout``."""
-    ys = _rows("ys", ys, plan.rows, plan)
-    dout = _rows("dout", dout, plan.tokens, plan)
-    H = ys.shape[1]
-    if dout.dtype != ys.dtype or dout.shape[1] != H:
+    ys, H, stride = _rows("ys", ys, plan.rows, plan)
+    dout, Hd, dstride = _rows("dout", dout, plan.tokens, plan)
+    if dout.dtype != ys.dtype or Hd != H:
         raise AffineBridgeError(
             f"dout must be [{plan.tokens}, {H}] {ys.dtype}, got {list(dout.shape)} {dout.dtype}")
     weights = _weights(weights, plan)
@@ -192,9 +191,8 @@ def moe_combine_backward(dout: torch.Tensor, ys: torch.Tensor, weights: torch.Te
     dw = weights.new_empty((plan.tokens, plan.top_k))
     ctx = Context.get(plan.device.index)
     st = L.load().mr_moe_combine_backward(
-        ctx.handle, dout.data_ptr(), _stride(dout), ys.data_ptr(), _stride(ys),
-        _ROW_DTYPES[ys.dtype], H, weights.data_ptr(), plan._ref, dys.data_ptr(), dw.data_ptr(),
-        _raw_stream(plan.device))
+        ctx.handle, dout.data_ptr(), dstride, ys.data_ptr(), stride, _ROW_DTYPES[ys.dtype], H,
+        weights.data_ptr(), plan._ref, dys.data_ptr(), dw.data_ptr(), _raw_stream(plan.device))
     if st:
         ctx.check("mr_moe_combine_backward", st)
     return dys, dw

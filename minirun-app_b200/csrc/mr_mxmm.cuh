@@ -52,11 +52,13 @@ constexpr int kMmK = 512;        // elements of a stage: with 256 the waits of o
                                  // cycles each, took longer than its MMAs
 constexpr int kMmMaxN = 176;     // activation rows of a tile: two accumulators and three
                                  // slots of exponents fit the 512 TMEM columns
-constexpr int kMmB = (kMmMaxN + 31) / 32;
+// Widest tile of a form, and its rows in groups of 32. (Code is fetched once a
+// kernel: a form without the other's unrolled rows starts 1-2 us earlier.)
+MR_DEVICE __host__ constexpr int mm_max_n(int cg) { return cg == 1 ? 64 : kMmMaxN; }
+MR_DEVICE __host__ constexpr int mm_max_b(int cg) { return (mm_max_n(cg) + 31) / 32; }
 constexpr int kMmThreads = 384;  // plus the gather warps
 constexpr int kMmGatherWarps = 4;  // sixteen warps in all: more would leave 96 registers each
 constexpr int kMmAPiece = kMmRows * 128;
-constexpr int kMmTokens = kMmThreads;  // rows whose tokens are looked up at the start
 constexpr int kMmRaw = 3;  // slots of the exponents' ring in shared memory
 
 // The MMAs' N, and a tile's width, step by 16.
@@ -89,7 +91,7 @@ struct MmMaps {
 // Shared memory: ring of codes, ring of exponents, barriers, group table.
 inline int mm_stage_bytes(int ntile, int cg) { return 2 * (kMmAPiece + ntile / cg * 128); }
 inline int mm_fixed_bytes(int E, int ntile) {
-  return 1024 + kMmRaw * mm_raw_rows(ntile) * 16 + 768 + 2 * (E + 1) * 4 + kMmTokens * 4;
+  return 1024 + kMmRaw * mm_raw_rows(ntile) * 16 + 768 + 2 * (E + 1) * 4;
 }
 
 // ------------------------------------------------------------ instructions
@@ -269,6 +271,15 @@ MR_DEVICE int mm_tiles(int n, int ntile) {
   return (int)((uint32_t)(n + w - 1) / w);
 }
 
+// Gathers of four rows that a CTA's half of a tile of n rows takes. The rest of
+// the half keeps what shared memory holds: those columns' results are not
+// kept. (Gathered as repeats of the last row, which 128 CTAs then read at
+// once, they made a single token's product 2 us slower; rows outside the
+// tensor, which read as zeros, a prefill 6 % slower.)
+MR_DEVICE int mm_quads(int n, int half, int rank) {
+  return (min(max(n - rank * half, 0), half) + 3) / 4;
+}
+
 // Walks the CTA's (or pair's) tiles in order: item -> expert, rows, and the
 // CTA's weight rows.
 template <int CG>
@@ -302,17 +313,15 @@ struct MmWalk {
 
 // ------------------------------------------------------------ exponents
 
-// The row of `a` that a pair takes its activations from. pair / top_k for pair
-// < 2^31: k_mul = ceil(2^(31 + k_shift) / top_k) with 2^k_shift >= top_k.
-MR_DEVICE int64_t mm_pair_row(const MmParams& p, int pair) {
-  const uint64_t t = ((uint64_t)(uint32_t)max(pair, 0) * p.k_mul) >> (31 + p.k_shift);
-  return min((int64_t)t, p.arows - 1);
-}
-// The same of sorted row r. Few rows have their tokens in shared memory.
-MR_DEVICE int64_t mm_act_row(const MmParams& p, const int* tok, int64_t r) {
-  if (!p.order) return min(r, p.arows - 1);
-  if (p.rows <= kMmTokens) return tok[r];
-  return mm_pair_row(p, __ldg(p.order + r));
+// The row of `a` that sorted row r takes its activations from.
+MR_DEVICE int64_t mm_act_row(const MmParams& p, int64_t r) {
+  if (p.order) {
+    // pair / top_k for pair < 2^31: k_mul = ceil(2^(31 + k_shift) / top_k) with
+    // 2^k_shift >= top_k
+    const int pair = max(__ldg(p.order + r), 0);
+    r = (int64_t)(((uint64_t)(uint32_t)pair * p.k_mul) >> (31 + p.k_shift));
+  }
+  return min(r, p.arows - 1);
 }
 
 // 16 bytes at an aligned address, of which only [lo, hi) may be read.
@@ -383,7 +392,7 @@ struct MmScaleRegs {
 template <int NB, bool WIDE, bool IS_A, int CG>
 MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lane, int first,
                               int stride, int n_items, uint4* raw, uint64_t* rfull,
-                              uint64_t* rempty, const int* tok, volatile int* flags) {
+                              uint64_t* rempty, volatile int* flags) {
   const int slot_rows = mm_raw_rows(p.ntile);
   const uint8_t* lo = IS_A ? p.w_scales : p.a_scales;
   const uint8_t* hi = lo + (IS_A ? (int64_t)p.E * p.out_features : p.arows) * p.groups;
@@ -395,12 +404,14 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lan
     const int have = IS_A ? kMmRows : it.n;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
+      src[i] = nullptr;
+      if (32 * i >= have) continue;
       // rows past the tile's end repeat its last: their results are not kept
       const int r = min(lane + 32 * i, have - 1);
       const int64_t row =
           IS_A ? (int64_t)it.e * p.out_features + min((int64_t)it.m0 + r, p.out_features - 1)
-               : mm_act_row(p, tok, (int64_t)it.row0 + r);
-      src[i] = 32 * i < have ? lo + row * p.groups : nullptr;
+               : mm_act_row(p, (int64_t)it.row0 + r);
+      src[i] = lo + row * p.groups;
     }
   };
   constexpr int kAhead = WIDE ? 2 : 1;  // registers of two unaligned stages would spill
@@ -479,7 +490,6 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   int* scan = reinterpret_cast<int*>(tslot + 2);  // [18] warp sums, [31] first tile's expert
   int* goff = scan + 32;
   int* gtile = goff + p.E + 1;
-  int* tok = gtile + p.E + 1;  // [kMmTokens]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = CG == 1 ? 0 : cluster_rank();
   const int first = blockIdx.x / CG, stride = gridDim.x / CG;
@@ -516,8 +526,6 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     scan[31] = 0;
   }
   const int tile0 = (int)((uint32_t)first / (uint32_t)p.mtiles);
-  if (p.order && p.rows <= kMmTokens && tid < p.rows)
-    tok[tid] = (int)mm_pair_row(p, __ldg(p.order + tid));
   for (int base = 0; base < p.E; base += kMmThreads) {
     const int e = base + tid;
     int a = 0, b = (int)p.rows, cnt = 0;
@@ -576,7 +584,8 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       const int half = mm_round(it.n) / CG;  // activation rows of this CTA
       const int ya = it.row0 + (int)rank * half;
       const int boxes = (half + p.box - 1) / p.box;
-      const uint32_t bytes = kMmAPiece + (p.order ? half : boxes * p.box) * 128;  // a piece
+      const int got = p.order ? 4 * mm_quads(it.n, half, (int)rank) : boxes * p.box;
+      const uint32_t bytes = kMmAPiece + got * 128;  // of a piece
       for (int st = 0; st < p.nstages; ++st, ++issued) {
         const int pieces = min(2, (p.groups - st * 16 + 7) / 8);
         wait_mbar(empty + slot, phase ^ 1u, flags, p.error);
@@ -661,13 +670,14 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     // ------------------------------------------- exponents to shared memory
     if (warp == 2)
       mm_load_scales<4, WIDE, true>(p, it, lane, first, stride, n_items, raw, rfull, rempty,
-                                    tok, flags);
+                                    flags);
     else
-      mm_load_scales<kMmB, WIDE, false>(p, it, lane, first, stride, n_items, raw, rfull,
-                                                rempty, tok, flags);
+      mm_load_scales<mm_max_b(CG), WIDE, false>(p, it, lane, first, stride, n_items, raw, rfull,
+                                                rempty, flags);
   } else if (warp >= 8 && warp < 12) {
     // -------------------------------------------- exponents to tensor memory
     const uint32_t lane_t = tbase + ((uint32_t)((warp & 3) * 32) << 16) + 2 * p.ntile;
+    constexpr int kB = mm_max_b(CG);
     const int sfc = mm_sf_cols(p.ntile), sfw = mm_sf_word(p.ntile);
     const int slot_rows = mm_raw_rows(p.ntile);
     uint32_t slot = 0, phase = 0, rslot = 0, rphase = 0;
@@ -676,11 +686,11 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         wait_mbar(rfull + rslot, rphase, flags, p.error);
         const bool free = mbar_test(empty + slot, phase ^ 1u);
         const uint4* src = raw + rslot * slot_rows + lane;
-        uint4 a[4], b[kMmB];  // rows lane + 32 i
+        uint4 a[4], b[kB];  // rows lane + 32 i
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = src[32 * i];
 #pragma unroll
-        for (int i = 0; i < kMmB; ++i)
+        for (int i = 0; i < kB; ++i)
           b[i] = 32 * i < p.ntile ? src[kMmRows + 32 * i] : make_uint4(0, 0, 0, 0);
         __syncwarp();
         if (lane == 0) mbar_arrive(rempty + rslot);
@@ -696,15 +706,15 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
 #pragma unroll
         for (int k = 0; k < 16; ++k) x[k] = word_of(a[k & 3], k >> 2);
         tmem_st16(t, x);
-        if (p.ntile > 128) {
+        if (CG == 2 && p.ntile > 128) {
           uint32_t y[32];
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            y[k] = (k & 7) < kMmB ? word_of(b[(k & 7) < kMmB ? k & 7 : 0], k >> 3) : 0u;
+            y[k] = (k & 7) < kB ? word_of(b[(k & 7) < kB ? k & 7 : 0], k >> 3) : 0u;
           tmem_st32(t + 16, y);
         } else {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[k] = word_of(b[k & 3], k >> 2);
+          for (int k = 0; k < 16; ++k) x[k] = (k & 3) < kB ? word_of(b[(k & 3) < kB ? k & 3 : 0], k >> 2) : 0u;
           tmem_st16(t + 16, x);
         }
         tmem_wait_st();
@@ -720,21 +730,21 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   } else if (warp >= 12) {
     // -------------------------------------------------------------- gathers
     if (!elect_one()) return;
-    constexpr int kMine = (kMmMaxN / CG / 4 + kMmGatherWarps - 1) / kMmGatherWarps;  // a piece's
+    constexpr int kMine = (mm_max_n(CG) / CG / 4 + kMmGatherWarps - 1) / kMmGatherWarps;
     const int w = warp - 12;
     uint32_t slot = 0, phase = 0;
     for (int item = first; item < n_items; item += stride) {
       it.at(item);
-      const int half = mm_round(it.n) / CG, nq = half / 4;
+      const int half = mm_round(it.n) / CG, nq = mm_quads(it.n, half, (int)rank);
       int4 rows[kMine];  // every kMmGatherWarps-th gather is this warp's
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
         if (w + i * kMmGatherWarps >= nq) break;
         const int r0 = it.row0 + (int)rank * half + 4 * (w + i * kMmGatherWarps);
-        const int r1 = it.row0 + it.n - 1;  // rows past the tile's end repeat its last
+        const int r1 = it.row0 + it.n - 1;  // a last gather of fewer than four repeats one
         rows[i] =
-            make_int4((int)mm_act_row(p, tok, min(r0, r1)), (int)mm_act_row(p, tok, min(r0 + 1, r1)),
-                      (int)mm_act_row(p, tok, min(r0 + 2, r1)), (int)mm_act_row(p, tok, min(r0 + 3, r1)));
+            make_int4((int)mm_act_row(p, min(r0, r1)), (int)mm_act_row(p, min(r0 + 1, r1)),
+                      (int)mm_act_row(p, min(r0 + 2, r1)), (int)mm_act_row(p, min(r0 + 3, r1)));
       }
       for (int st = 0; st < p.nstages; ++st) {
         const int pieces = min(2, (p.groups - st * 16 + 7) / 8);

@@ -19,6 +19,7 @@ from .mxfp4_scaled import (mxfp4_grouped_mm, mxfp4_quantize, mxfp4_quantize_swig
                            mxfp4_scaled_mm)
 from .sorted_tokens import (SortedTokens, moe_combine, moe_combine_backward, moe_dispatch,
                             moe_dispatch_backward, moe_sort)
+from .mxfp4_moe import MXFP4MoELayer
 from .k3 import K3MoE, K3Projection, dense_mm_f32, situ
 from .tiles import (ExpertContainers, TileContainer, TileContainerError, write_container,
                     write_expert_containers)
@@ -35,5 +36,5 @@ __all__ = [
     "mxfp4_gather_mm_f32", "mxfp4_mm_f32", "K3MoE", "K3Projection", "dense_mm_f32", "situ",
     "mxfp4_quantize", "mxfp4_quantize_swiglu", "mxfp4_scaled_mm", "mxfp4_grouped_mm",
     "SortedTokens", "moe_sort", "moe_dispatch", "moe_dispatch_backward", "moe_combine",
-    "moe_combine_backward",
+    "moe_combine_backward", "MXFP4MoELayer",
 ]

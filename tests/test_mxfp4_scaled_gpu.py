@@ -347,3 +347,63 @@ def test_refusals():
     odd = torch.empty(4 * 8 + 1, dtype=torch.int32, device=dev())[1:].view(4, 8)
     with pytest.raises(M.MoeError, match="16-byte aligned"):
         M.mxfp4_scaled_mm(M.MXFP4Weights(odd, a.scales), w)
+
+
+@pytest.mark.parametrize("T,shared,limit", [(1, False, 0.0), (37, True, 0.0), (300, True, 2.0)])
+def test_layer_is_its_steps_in_64_bits(T, shared, limit):
+    """MXFP4MoELayer against the same steps in fp64 on the same weights. The layer rounds the
+    gate/up result to bf16 and the hidden values to 4 bits, so fp64 takes its hidden codes from
+    the layer's own gate/up values; the rest is held to the bf16 rounding of ys, the shared rows
+    and the sum, 3 * 2^-8 of the magnitudes added."""
+    E, k, H, I = 8, 3, 256, 128
+    g = torch.Generator().manual_seed(T)
+    rnd = lambda *s: (torch.randn(s, generator=g) / s[-1] ** 0.5).to(dev())  # noqa: E731
+    router_w = rnd(E, H).bfloat16()
+    dense_w = (rnd(E, I, H), rnd(E, I, H), rnd(E, H, I))
+    sh = (rnd(2 * I, H), rnd(2 * I, H), rnd(H, 2 * I)) if shared else None
+    layer = M.MXFP4MoELayer.from_dense(router_w, *dense_w, M.RouterConfig.qwen(E, k), shared=sh,
+                                       swiglu_limit=limit)
+    x = torch.randn((T, H), generator=g).bfloat16().to(dev())
+    out, sel = layer(x)
+
+    def mlp(gu, dn, rows):  # one expert on 4-bit rows, its gate/up rounded as the kernel's
+        mid = torch.from_numpy(rows @ gu.T).to(torch.bfloat16).double().numpy()
+        a, u = mid[:, :mid.shape[1] // 2], mid[:, mid.shape[1] // 2:]
+        if limit:
+            a, u = np.minimum(a, limit), np.clip(u, -limit, limit)
+        h = np_values(*np_quantize(a / (1 + np.exp(-a)) * u))
+        return h @ dn.T, np.abs(h) @ np.abs(dn).T
+
+    X = dense(M.mxfp4_quantize(x))
+    G, D = dense(layer.gate_up), dense(layer.down)
+    ids, wt = sel.ids.cpu().numpy(), sel.weights.double().cpu().numpy()
+    ref, mag = np.zeros((T, H)), np.zeros((T, H))
+    for t in range(T):
+        for j in range(k):
+            y, m = mlp(G[ids[t, j]], D[ids[t, j]], X[t:t + 1])
+            ref[t] += wt[t, j] * y[0]
+            mag[t] += wt[t, j] * m[0]
+    if shared:
+        y, m = mlp(dense(layer.shared[0]), dense(layer.shared[1]), X)
+        ref, mag = ref + y, mag + m
+    err = np.abs(out.double().cpu().numpy() - ref)
+    # a gate/up sum next to a bf16 or 4-bit rounding boundary may fall the other way in fp64:
+    # one code step of one hidden value then, at most 2 / 6 of its block's largest number
+    within = err <= 3 * 2.0 ** -8 * mag
+    assert within.mean() > 0.99, within.mean()
+    assert np.linalg.norm(err) <= 2.0 ** -7 * np.linalg.norm(ref)
+
+
+def test_layer_refusals():
+    E, H, I = 4, 64, 32
+    r = M.RouterConfig.qwen(E, 2)
+    gu, dn = weights(2 * I, H, 1, experts=E), weights(H, I, 2, experts=E)
+    rw = torch.zeros((E, H), dtype=torch.bfloat16, device=dev())
+    layer = M.MXFP4MoELayer(rw, gu, dn, r)
+    for f in (lambda: M.MXFP4MoELayer(rw, dn, gu, r),
+              lambda: M.MXFP4MoELayer(rw, gu, weights(H, I, 2, experts=3), r),
+              lambda: M.MXFP4MoELayer(rw, gu, dn, r, shared=(gu, dn)),
+              lambda: M.MXFP4MoELayer(rw, gu, dn, r, swiglu_limit=-1.0),
+              lambda: layer(torch.zeros((2, H), device=dev()))):
+        with pytest.raises(M.AffineBridgeError):
+            f()

@@ -90,28 +90,43 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
   const bool wide =
       p.groups % 16 == 0 && addr(w->scales) % 16 == 0 && addr(a->scales) % 16 == 0;
   // Tile width: twice an expert's mean rows, so that few experts need a
-  // second tile; narrow tiles leave room for a deeper ring.
+  // second tile; narrow tiles leave room for a deeper ring. Tiles are at most
+  // one per expert with rows and the full ones.
   const int64_t mean = plan ? (rows + p.E - 1) / p.E : rows;
   const int64_t want = plan ? std::min(rows, 2 * mean) : rows;
+  const int sms = ctx->sm_count;
+  auto tiles_of = [&](int ntile, int cg) {
+    return (std::min<int64_t>(p.E, rows) + (rows - 1) / ntile) *
+           ((w->out_features + kMmRows * cg - 1) / (kMmRows * cg));
+  };
   p.ntile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : kMmMaxN;
   const int cg = p.ntile > 64 ? 2 : 1;
+  const int64_t tiles = tiles_of(p.ntile, cg);
+  if (tiles > INT32_MAX)
+    return fail(ctx, MR_ERR_UNSUPPORTED, "the product has more than 2^31 tiles");
+  p.ksplit = 1;
+  // CTAs share a tile where there are few, the rows are long and the tile is
+  // narrow (1 and 16 rows x 2048 x 7168: 8.2 -> 6.2 us and 8.1 -> 6.8; with 32
+  // rows, or rows of 2048, the exchange costs what the shorter loop saves).
+  while (p.ntile == 16 && p.ksplit < kMmSplit && 2 * p.ksplit * tiles <= sms && p.nstages >= 8)
+    p.ksplit *= 2;
   p.mtiles = (int)((w->out_features + kMmRows * cg - 1) / (kMmRows * cg));
   p.box = p.order ? 1 : p.ntile > 32 ? p.ntile / 2 : p.ntile;
-  const int fixed = mm_fixed_bytes(p.E, p.ntile);
+  const int fixed = mm_fixed_bytes(p.E, p.ntile, p.ksplit);
   p.nst = std::min((512 - 2 * p.ntile) / mm_sf_cols(p.ntile),
                    (kMmSmem - fixed) / mm_stage_bytes(p.ntile, cg));
-  const int smem = fixed + p.nst * mm_stage_bytes(p.ntile, cg);
+  const int used = fixed + p.nst * mm_stage_bytes(p.ntile, cg);
+  const int part = p.ksplit > 1 ? p.ntile * kMmRows * 4 : 0;
+  p.part_at = (used - 1024 - part) & ~15;  // the last bytes; the first 1024 are for alignment
+  const int smem = used;
 
   MmMaps maps;
   const int64_t bytes = w->in_features / 2;
   if (!encode_codes(&maps.w, w->packed, (int64_t)p.E * w->out_features, bytes, kMmRows) ||
       !encode_codes(&maps.a, a->packed, a->out_features, bytes, p.box))
     return fail(ctx, MR_ERR_UNSUPPORTED, "cannot describe the operands as tensor maps");
-  // at most one row tile per expert plus the full ones
-  const int64_t tiles = (std::min<int64_t>(p.E, rows) + rows / p.ntile) * p.mtiles;
-  if (tiles > INT32_MAX)
-    return fail(ctx, MR_ERR_UNSUPPORTED, "the product has more than 2^31 tiles");
-  const int grid = (int)std::min<int64_t>(ctx->sm_count / cg, tiles) * cg;
+  const int unit = cg * p.ksplit;  // CTAs that work together
+  const int grid = (int)std::min<int64_t>(sms / unit, tiles) * unit;
   const int threads = kMmThreads + (p.order ? 32 * kMmGatherWarps : 0);
   auto* kernel = cg == 1 ? (wide ? mxmm_kernel<true, 1> : mxmm_kernel<false, 1>)
                          : (wide ? mxmm_kernel<true, 2> : mxmm_kernel<false, 2>);
@@ -125,7 +140,7 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cg;
+    attr[1].val.clusterDim.x = unit;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};

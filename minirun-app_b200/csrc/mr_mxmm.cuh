@@ -14,6 +14,11 @@
 // leader's MMAs (cta_group::2) read both halves: per MMA a CTA takes 28 KB
 // from L2 instead of 40.
 //
+// Where there are few narrow tiles (CG = 1), a cluster of `ksplit` CTAs shares each:
+// every CTA multiplies its part of the row's stages and leaves the partial
+// result in its shared memory, and each then sums a share of the columns over
+// the cluster, always in the order of the parts.
+//
 // Persistent CTAs (or pairs) loop over tiles (expert's row tile x weight
 // rows, the weight rows fastest, so that CTAs working side by side share
 // activations). Per stage of 512 elements (256 bytes of codes a row, as two
@@ -59,6 +64,7 @@ MR_DEVICE __host__ constexpr int mm_max_b(int cg) { return (mm_max_n(cg) + 31) /
 constexpr int kMmThreads = 384;  // plus the gather warps
 constexpr int kMmGatherWarps = 4;  // sixteen warps in all: more would leave 96 registers each
 constexpr int kMmAPiece = kMmRows * 128;
+constexpr int kMmSplit = 4;  // CTAs that share a tile's stages, at most
 constexpr int kMmRaw = 3;  // slots of the exponents' ring in shared memory
 
 // The MMAs' N, and a tile's width, step by 16.
@@ -82,6 +88,8 @@ struct MmParams {
   int groups;           // in / 32
   int nstages, mtiles;
   int ntile, box, nst;  // tile width, rows of an activation box, ring stages
+  int ksplit;           // CTAs that share a tile's stages
+  int part_at;          // where the partial result lies in shared memory
   int out_f32;
 };
 struct MmMaps {
@@ -90,8 +98,9 @@ struct MmMaps {
 
 // Shared memory: ring of codes, ring of exponents, barriers, group table.
 inline int mm_stage_bytes(int ntile, int cg) { return 2 * (kMmAPiece + ntile / cg * 128); }
-inline int mm_fixed_bytes(int E, int ntile) {
-  return 1024 + kMmRaw * mm_raw_rows(ntile) * 16 + 768 + 2 * (E + 1) * 4;
+inline int mm_fixed_bytes(int E, int ntile, int ksplit) {
+  return 1024 + kMmRaw * mm_raw_rows(ntile) * 16 + 768 + 2 * (E + 1) * 4 +
+         (ksplit > 1 ? ntile * kMmRows * 4 : 0);
 }
 
 // ------------------------------------------------------------ instructions
@@ -220,6 +229,28 @@ MR_DEVICE void mm_arrive(uint64_t* bar, uint32_t to, uint32_t rank) {
         : "memory");
   }
 }
+// Partial sums: made visible to the cluster, and read from another CTA.
+MR_DEVICE void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+MR_DEVICE uint32_t at_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+MR_DEVICE float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+// Arrive (relaxed: after fence_cluster) on this barrier of every CTA.
+MR_DEVICE void arrive_all(uint64_t* bar, int ctas) {
+  for (int c = 0; c < ctas; ++c)
+    asm volatile(
+        "{ .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n"
+        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [r]; }" ::"r"(smem_u32(bar)),
+        "r"(c)
+        : "memory");
+}
+
 // wait_bounded as one look at the barrier and a call where that is not
 // enough: sixteen warps run different code, and its size costs each of them.
 // One lane of a warp waits alone only where the others have left; elsewhere
@@ -391,8 +422,8 @@ struct MmScaleRegs {
 // pipeline. A slot holds 16 bytes a row. Every lane of the warp.
 template <int NB, bool WIDE, bool IS_A, int CG>
 MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lane, int first,
-                              int stride, int n_items, uint4* raw, uint64_t* rfull,
-                              uint64_t* rempty, volatile int* flags) {
+                              int stride, int n_items, int st0, int st1, uint4* raw,
+                              uint64_t* rfull, uint64_t* rempty, volatile int* flags) {
   const int slot_rows = mm_raw_rows(p.ntile);
   const uint8_t* lo = IS_A ? p.w_scales : p.a_scales;
   const uint8_t* hi = lo + (IS_A ? (int64_t)p.E * p.out_features : p.arows) * p.groups;
@@ -426,13 +457,13 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lan
         v[b].off[i] = 0;
       }
     }
-  int litem = first, lq = 0;  // the stage to load next
+  int litem = first, lq = st0;  // the stage to load next
   open(litem);
   auto load = [&](MmScaleRegs<NB, WIDE>& r) {
     if (litem >= n_items) return;
     r.load(src, lq, p.groups, lo, hi);
-    if (++lq == p.nstages) {
-      lq = 0;
+    if (++lq == st1) {
+      lq = st0;
       litem += stride;
       open(litem);
     }
@@ -440,7 +471,7 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lan
 #pragma unroll
   for (int b = 0; b < kAhead; ++b) load(v[b]);
   uint32_t slot = 0, phase = 0;
-  int item = first, q = 0;  // the stage to hand on next
+  int item = first, q = st0;  // the stage to hand on next
   while (item < n_items) {
 #pragma unroll
     for (int b = 0; b < kAhead; ++b) {
@@ -457,8 +488,8 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lan
         phase ^= 1u;
       }
       load(v[b]);
-      if (++q == p.nstages) {
-        q = 0;
+      if (++q == st1) {
+        q = st0;
         item += stride;
       }
     }
@@ -485,14 +516,21 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   uint64_t* drain = dempty + 2;       // every MMA complete
   uint64_t* done = drain + 1;         // every other access of TMEM too
   uint64_t* bye = done + 1;           // the other CTA needs this one's memory no more
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(bye + 1);
+  uint64_t* pfull = bye + 1;          // every CTA's partial result is there (ksplit > 1)
+  uint64_t* pempty = pfull + 1;       // this CTA's has been read by all
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(pempty + 1);
   volatile int* flags = reinterpret_cast<volatile int*>(tslot + 1);
   int* scan = reinterpret_cast<int*>(tslot + 2);  // [18] warp sums, [31] first tile's expert
   int* goff = scan + 32;
   int* gtile = goff + p.E + 1;
+  // [ntile][128] this CTA's partial result, 16-byte aligned: after the ring
+  float* part = reinterpret_cast<float*>(smem + p.part_at);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = CG == 1 ? 0 : cluster_rank();
-  const int first = blockIdx.x / CG, stride = gridDim.x / CG;
+  const int ks = CG == 1 ? p.ksplit : 1;
+  const int kpart = ks > 1 ? (int)cluster_rank() : 0;
+  const int st0 = p.nstages * kpart / ks, st1 = p.nstages * (kpart + 1) / ks;
+  const int first = blockIdx.x / (CG * ks), stride = gridDim.x / (CG * ks);
   // the leader's copies complete on `full` itself, the other CTA's on a
   // barrier of its own, whose arrival is passed on
   uint64_t* cfull = rank == 0 ? full : lfull;
@@ -513,6 +551,8 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     mbar_init(drain, 1);
     mbar_init(done, rank == 0 ? 8 : 9);
     mbar_init(bye, 1);
+    mbar_init(pfull, 4 * ks);
+    mbar_init(pempty, 4 * ks);
     flags[0] = 0;
     fence_mbar_init();
   }
@@ -565,10 +605,10 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     if (base + kMmThreads < p.E) __syncthreads();
   }
   tc_fence_before();
-  if constexpr (CG == 1)
+  if (CG * ks == 1)
     __syncthreads();
   else
-    cooperative_groups::this_cluster().sync();  // the other CTA's barriers are there too
+    cooperative_groups::this_cluster().sync();  // the other CTAs' barriers are there too
   tc_fence_after();
   constexpr uint32_t tbase = 0;  // all 512 columns are this CTA's: they start at 0
   const int n_items = gtile[p.E] * p.mtiles;
@@ -586,7 +626,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       const int boxes = (half + p.box - 1) / p.box;
       const int got = p.order ? 4 * mm_quads(it.n, half, (int)rank) : boxes * p.box;
       const uint32_t bytes = kMmAPiece + got * 128;  // of a piece
-      for (int st = 0; st < p.nstages; ++st, ++issued) {
+      for (int st = st0; st < st1; ++st, ++issued) {
         const int pieces = min(2, (p.groups - st * 16 + 7) / 8);
         wait_mbar(empty + slot, phase ^ 1u, flags, p.error);
         mbar_arrive_expect_tx(cfull + slot, pieces * bytes);
@@ -617,7 +657,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       // this CTA's copies have landed: tell the leader
       uint32_t slot = 0, phase = 0;
       for (int item = first; item < n_items; item += stride)
-        for (int st = 0; st < p.nstages; ++st) {
+        for (int st = st0; st < st1; ++st) {
           wait_mbar(lfull + slot, phase, flags, p.error);
           mm_arrive<CG>(full + slot, 0, rank);
           if (++slot == (uint32_t)nst) {
@@ -638,7 +678,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       const uint32_t id0 = umma_idesc_mxf4<CG>(nn, 0), id1 = umma_idesc_mxf4<CG>(nn, 1);
       wait_mbar(dempty + db, ((t >> 1) & 1u) ^ 1u, flags, p.error);
       const uint32_t d_t = db * p.ntile;
-      for (int st = 0; st < p.nstages; ++st) {
+      for (int st = st0; st < st1; ++st) {
         const uint32_t sfa = 2 * p.ntile + slot * sfc, sfb = sfa + 16;
         const uint64_t ad = ad0 + slot * (2 * kMmAPiece >> 4), bd = bd0 + slot * (2 * b_piece >> 4);
         wait_mbar(full + slot, phase, flags, p.error);
@@ -648,7 +688,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         auto mma = [&](int kk) {
           tc_mma_mxf4<CG>(d_t, ad + ((kk >> 2) * (kMmAPiece >> 4) + (kk & 3) * 2),
                           bd + ((kk >> 2) * (b_piece >> 4) + (kk & 3) * 2), (kk & 1) ? id1 : id0,
-                          sfa + 4 * (kk >> 1), sfb + sfw * (kk >> 1), (st | kk) ? 1u : 0u);
+                          sfa + 4 * (kk >> 1), sfb + sfw * (kk >> 1), (st > st0 || kk > 0) ? 1u : 0u);
         };
         if (steps == 8) {
 #pragma unroll
@@ -669,11 +709,11 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   } else if (warp < 4) {
     // ------------------------------------------- exponents to shared memory
     if (warp == 2)
-      mm_load_scales<4, WIDE, true>(p, it, lane, first, stride, n_items, raw, rfull, rempty,
-                                    flags);
+      mm_load_scales<4, WIDE, true>(p, it, lane, first, stride, n_items, st0, st1, raw, rfull,
+                                    rempty, flags);
     else
-      mm_load_scales<mm_max_b(CG), WIDE, false>(p, it, lane, first, stride, n_items, raw, rfull,
-                                                rempty, flags);
+      mm_load_scales<mm_max_b(CG), WIDE, false>(p, it, lane, first, stride, n_items, st0, st1,
+                                                       raw, rfull, rempty, flags);
   } else if (warp >= 8 && warp < 12) {
     // -------------------------------------------- exponents to tensor memory
     const uint32_t lane_t = tbase + ((uint32_t)((warp & 3) * 32) << 16) + 2 * p.ntile;
@@ -682,7 +722,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     const int slot_rows = mm_raw_rows(p.ntile);
     uint32_t slot = 0, phase = 0, rslot = 0, rphase = 0;
     for (int item = first; item < n_items; item += stride)
-      for (int st = 0; st < p.nstages; ++st) {
+      for (int st = st0; st < st1; ++st) {
         wait_mbar(rfull + rslot, rphase, flags, p.error);
         const bool free = mbar_test(empty + slot, phase ^ 1u);
         const uint4* src = raw + rslot * slot_rows + lane;
@@ -746,7 +786,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
             make_int4((int)mm_act_row(p, min(r0, r1)), (int)mm_act_row(p, min(r0 + 1, r1)),
                       (int)mm_act_row(p, min(r0 + 2, r1)), (int)mm_act_row(p, min(r0 + 3, r1)));
       }
-      for (int st = 0; st < p.nstages; ++st) {
+      for (int st = st0; st < st1; ++st) {
         const int pieces = min(2, (p.groups - st * 16 + 7) / 8);
         wait_mbar(empty + slot, phase ^ 1u, flags, p.error);
         for (int k = 0; k < pieces; ++k) {
@@ -775,6 +815,59 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       tc_fence_after();
       const int64_t o = it.m0 + q * 32 + lane;
       const uint32_t d_t = tbase + db * p.ntile + ((uint32_t)(q * 32) << 16);
+      if (ks > 1) {
+        const int row = q * 32 + lane;
+        wait_mbar(pempty, (t & 1u) ^ 1u, flags, p.error);
+        for (int c = 0; c < it.n; c += 16) {
+          float v[16];
+          tmem_ld16(d_t + c, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) part[(c + i) * kMmRows + row] = v[i];
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(dempty + db);
+          fence_cluster();
+          arrive_all(pfull, ks);
+        }
+        __syncwarp();
+        wait_mbar(pfull, t & 1u, flags, p.error);
+        fence_cluster();
+        // this CTA's share of the columns, four at a time: all parts' loads first
+        const int share = (it.n + ks - 1) / ks, c1 = min(it.n, (kpart + 1) * share);
+        uint32_t from[kMmSplit];
+#pragma unroll
+        for (int k = 0; k < kMmSplit; ++k)
+          from[k] = at_rank(smem_u32(part + row), k < ks ? k : 0);
+        for (int c = kpart * share; c < c1; c += 4) {
+          float x[4][kMmSplit];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int k = 0; k < kMmSplit; ++k)
+              x[j][k] = k < ks && c + j < c1 ? ld_cluster(from[k] + (c + j) * kMmRows * 4) : 0.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float sum = x[j][0];
+#pragma unroll
+            for (int k = 1; k < kMmSplit; ++k) sum += x[j][k];
+            if (c + j >= c1 || o >= p.out_features) continue;
+            const int64_t to = ((int64_t)it.row0 + c + j) * p.out_features + o;
+            if (p.out_f32)
+              put(reinterpret_cast<float*>(p.out) + to, sum);
+            else
+              put(reinterpret_cast<uint16_t*>(p.out) + to, sum);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          fence_cluster();
+          arrive_all(pempty, ks);
+        }
+        __syncwarp();
+        continue;
+      }
       for (int c = 0; c < it.n; c += 16) {
         float v[16];
         tmem_ld16(d_t + c, v);
@@ -789,6 +882,8 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       __syncwarp();
       if (lane == 0) mm_arrive<CG>(dempty + db, 0, rank);
     }
+    // every CTA has read this one's last partial result
+    if (ks > 1 && t > 0) wait_mbar(pempty, (t - 1) & 1u, flags, p.error);
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(done);

@@ -196,6 +196,21 @@ def test_scaled_mm(rows, out, inn, out_dtype):
     assert M.Context.get(0).sync_check() == 0
 
 
+@pytest.mark.parametrize("rows,out,inn", [
+    (1, 130, 2048), (5, 2048, 7168), (64, 300, 4096), (70, 256, 2080), (100, 1000, 4096),
+    (33, 128, 8160),
+])
+def test_scaled_mm_few_tiles_split_along_the_rows(rows, out, inn):
+    """Long rows and few tiles: several CTAs share one, and always add up alike."""
+    a, w = weights(rows, inn, rows + 3), weights(out, inn, out + 4)
+    A, W = dense(a), dense(w)
+    for dt in (torch.bfloat16, torch.float32):
+        y = M.mxfp4_scaled_mm(a, w, out_dtype=dt)
+        check_mm(y, A @ W.T, np.abs(A) @ np.abs(W).T, inn)
+        assert torch.equal(y, M.mxfp4_scaled_mm(a, w, out_dtype=dt))
+    assert M.Context.get(0).sync_check() == 0
+
+
 def grouped(T, k, E, out, inn, by_token, seed=0, dropped=0.0, ids=None, out_dtype=torch.bfloat16):
     rng = np.random.default_rng(seed)
     if ids is None:
@@ -220,7 +235,7 @@ def grouped(T, k, E, out, inn, by_token, seed=0, dropped=0.0, ids=None, out_dtyp
 @pytest.mark.parametrize("T,k,E,out,inn,dropped", [
     (1, 8, 256, 128, 512, 0.0), (5, 2, 4, 200, 288, 0.0), (64, 8, 40, 136, 256, 0.0),
     (300, 4, 6, 256, 1024, 0.3), (40, 6, 1024, 64, 64, 0.0), (700, 2, 3, 130, 2048, 0.0),
-    (9, 3, 5, 128, 96, 1.0),
+    (9, 3, 5, 128, 96, 1.0), (2, 1, 3, 256, 4096, 0.0), (3, 2, 4, 100, 6144, 0.3),
 ])
 def test_grouped_mm(T, k, E, out, inn, dropped, by_token):
     grouped(T, k, E, out, inn, by_token, seed=T, dropped=dropped)

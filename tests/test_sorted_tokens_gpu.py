@@ -27,7 +27,7 @@ def dev():
 def choice(T, k, E, seed, dropped=0.0, distinct=True):
     rng = np.random.default_rng(seed)
     if distinct and k <= E:
-        ids = np.stack([rng.permutation(E)[:k] for _ in range(T)]) if T else np.zeros((0, k))
+        ids = np.argsort(rng.random((T, E), dtype=np.float32), axis=1)[:, :k]
     else:
         ids = rng.integers(0, E, size=(T, k))
     ids = ids.astype(np.int32).reshape(T, k)
@@ -37,12 +37,13 @@ def choice(T, k, E, seed, dropped=0.0, distinct=True):
 
 def np_plan(ids, E):
     flat = ids.reshape(-1)
-    kept = [p for e in range(E) for p in np.nonzero(flat == e)[0]]
+    key = np.where((flat >= 0) & (flat < E), flat, E)
+    kept = np.argsort(key, kind="stable")[:(key < E).sum()]
     order = np.full(flat.size, -1, np.int32)
     order[:len(kept)] = kept
     inverse = np.full(flat.size, -1, np.int32)
     inverse[kept] = np.arange(len(kept))
-    counts = np.array([(flat == e).sum() for e in range(E)])
+    counts = np.bincount(key, minlength=E + 1)[:E]
     return order, inverse.reshape(ids.shape), np.concatenate([[0], np.cumsum(counts)])
 
 
@@ -67,7 +68,7 @@ def within(got, ref, mag, n, dtype):
 PLANS = [  # tokens, top_k, experts, dropped share
     (1, 1, 1, 0.0), (1, 8, 256, 0.0), (3, 2, 5, 0.5), (64, 8, 256, 0.0), (33, 4, 1024, 0.3),
     (513, 8, 60, 0.0), (512, 8, 61, 0.0), (4097, 3, 7, 0.2), (9001, 8, 256, 0.0),
-    (700, 6, 1024, 1.0), (5, 32, 40, 0.1),
+    (700, 6, 1024, 1.0), (5, 32, 40, 0.1), (30011, 8, 1024, 0.1), (200003, 2, 3, 0.0),
 ]
 
 

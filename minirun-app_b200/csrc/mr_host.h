@@ -20,12 +20,24 @@ inline mr_status guarded(F&& f) {
   }
 }
 
-// The context's device, for callers whose current device is another one.
-inline cudaError_t set_device(const mr_ctx* ctx) {
-  int cur = -1;
-  const cudaError_t e = cudaGetDevice(&cur);
-  return e == cudaSuccess && cur != ctx->device ? cudaSetDevice(ctx->device) : e;
-}
+// The context's device is current while this lives; the caller's is afterwards.
+struct DeviceScope {
+  int prev = -1;
+  cudaError_t err;
+  explicit DeviceScope(const mr_ctx* ctx) {
+    int cur = -1;
+    err = cudaGetDevice(&cur);
+    if (err == cudaSuccess && cur != ctx->device) {
+      err = cudaSetDevice(ctx->device);
+      prev = cur;
+    }
+  }
+  ~DeviceScope() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
 
 // Sets a kernel's attributes the first time a context launches it.
 enum KernelAttr : unsigned {

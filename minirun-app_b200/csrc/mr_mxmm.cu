@@ -130,7 +130,8 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
   const int threads = kMmThreads + (p.order ? 32 * kMmGatherWarps : 0);
   auto* kernel = cg == 1 ? (wide ? mxmm_kernel<true, 1> : mxmm_kernel<false, 1>)
                          : (wide ? mxmm_kernel<true, 2> : mxmm_kernel<false, 2>);
-  cudaError_t e = set_device(ctx);
+  const DeviceScope on(ctx);
+  cudaError_t e = on.err;
   if (e == cudaSuccess)
     e = attrs_once(ctx, kAttrProduct << (2 * (cg - 1) + wide), [&] {
       return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmSmem);

@@ -229,7 +229,8 @@ mr_status quantize(mr_ctx* ctx, const void* x, mr_dtype dt, int64_t rows, int64_
                 rows * (width / 8), packed, scales, values, limit};
   const bool aligned = addr(x) % 16 == 0 && (p.stride % 16 == 0 || rows == 1);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = set_device(ctx);
+  const DeviceScope on(ctx);
+  cudaError_t e = on.err;
   if (e == cudaSuccess)
     e = dt == MR_DTYPE_BF16  ? launch_q<MR_DTYPE_BF16>(ctx, p, aligned, swiglu, s)
         : dt == MR_DTYPE_F16 ? launch_q<MR_DTYPE_F16>(ctx, p, aligned, swiglu, s)

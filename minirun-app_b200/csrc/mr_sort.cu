@@ -628,7 +628,8 @@ mr_status combine_rows(mr_ctx* ctx, const void* ys, mr_dtype dt, int64_t stride,
   p.weights = weights;
   const dim3 grid = row_grid(ctx, p);
   cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
-  cudaError_t e = set_device(ctx);
+  const DeviceScope on(ctx);
+  cudaError_t e = on.err;
   if (e == cudaSuccess)
     e = dt == MR_DTYPE_BF16  ? launch_combine<MR_DTYPE_BF16>(p, vb, grid, cs)
         : dt == MR_DTYPE_F16 ? launch_combine<MR_DTYPE_F16>(p, vb, grid, cs)
@@ -685,7 +686,8 @@ mr_status mr_moe_sort(mr_ctx* ctx, const int32_t* ids, int64_t tokens, int32_t t
     const int64_t per = (p.P + (int64_t)ctas * warps - 1) / ((int64_t)ctas * warps);
     p.chunk = (per + 31) / 32 * 32;
     const size_t smem = sizeof(int) * ((size_t)warps * experts + 2 * experts + 32);
-    cudaError_t e = set_device(ctx);
+    const DeviceScope on(ctx);
+    cudaError_t e = on.err;
     if (e == cudaSuccess)
       e = attrs_once(ctx, kAttrSort, [] {
         const cudaError_t a = cudaFuncSetAttribute(
@@ -730,7 +732,8 @@ mr_status mr_moe_dispatch(mr_ctx* ctx, const void* x, mr_dtype dtype, int64_t x_
     p.dst = static_cast<char*>(xs);
     const dim3 grid = row_grid(ctx, p);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = set_device(ctx);
+    const DeviceScope on(ctx);
+    cudaError_t e = on.err;
     if (e == cudaSuccess)
       e = vb == 16  ? launch_pdl(dispatch_kernel<16>, grid, kRowThreads, 0, s, p)
           : vb == 8 ? launch_pdl(dispatch_kernel<8>, grid, kRowThreads, 0, s, p)
@@ -795,7 +798,8 @@ mr_status mr_moe_combine_backward(mr_ctx* ctx, const void* dout, int64_t dout_st
            p.T * p.group / kRowThreads * ((p.k + 2 * jn - 1) / (2 * jn)) >= 4 * ctx->sm_count)
       jn *= 2;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    cudaError_t e = set_device(ctx);
+    const DeviceScope on(ctx);
+    cudaError_t e = on.err;
     if (e == cudaSuccess)
       e = dtype == MR_DTYPE_BF16  ? launch_bwd_of<MR_DTYPE_BF16>(p, vb, jn, s)
           : dtype == MR_DTYPE_F16 ? launch_bwd_of<MR_DTYPE_F16>(p, vb, jn, s)

@@ -241,3 +241,33 @@ def load():
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+# The functions of csrc/mr_torch.cpp's bind, in its order.
+_TORCH_API = ("mr_moe_sort", "mr_moe_dispatch", "mr_moe_dispatch_backward", "mr_moe_combine",
+              "mr_moe_combine_backward", "mr_mxfp4_quantize", "mr_mxfp4_quantize_swiglu",
+              "mr_mxfp4_scaled_mm", "mr_mxfp4_grouped_mm")
+TORCH_PATH = os.path.join(_HERE, "_lib", "_minirun_torch.so")
+_torch_ext = None
+
+
+def load_torch():
+    """The module that takes torch tensors straight to the library (csrc/mr_torch.cpp), bound to
+    the loaded library. Raises LibraryMissing if it was not built."""
+    global _torch_ext
+    if _torch_ext is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries first)
+        if not os.path.exists(TORCH_PATH):
+            raise LibraryMissing(f"{TORCH_PATH} is missing: build it with "
+                                 "`make -C minirun-app_b200/csrc`")
+        loader = importlib.machinery.ExtensionFileLoader("_minirun_torch", TORCH_PATH)
+        ext = importlib.util.module_from_spec(
+            importlib.util.spec_from_loader("_minirun_torch", loader))
+        loader.exec_module(ext)
+        lib = load()
+        ext.bind(*(C.cast(getattr(lib, n), vp).value for n in _TORCH_API))
+        _torch_ext = ext
+    return _torch_ext

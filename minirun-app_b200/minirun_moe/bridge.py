@@ -51,6 +51,7 @@ class Context:
         if st != L.MR_OK:
             raise MoeError("mr_ctx_create", st, "cannot create a context on device %d" % device)
         self.handle = h
+        self.address = h.value
         self.device = device
 
     def __del__(self):

@@ -53,6 +53,14 @@ def mxfp4_quantize(x: torch.Tensor, values: bool = False):
     """``x`` [rows, in] or [experts, rows, in] in MXFP4 (see mr_mxfp4_quantize for the rounding).
     With ``values`` the pair (codes, values): the numbers the codes stand for in x's type, what a
     training step with 4-bit forward values multiplies with."""
+    if x.is_cuda and x.dim() == 2:
+        ctx = Context.get(x.get_device())
+        r = L.load_torch().quantize(ctx.address, ctx.device, x, values)
+        if r is not None:
+            if r.__class__ is int:
+                ctx.check("mr_mxfp4_quantize", r)
+            q = _weights_of(r[0], r[1], x.shape[0], x.shape[1], None)
+            return (q, r[2]) if values else q
     x, shape, stride = _checked("x", x)
     if len(shape) == 2:
         experts, (rows, width) = None, shape
@@ -82,6 +90,13 @@ def mxfp4_quantize(x: torch.Tensor, values: bool = False):
 def mxfp4_quantize_swiglu(gate_up: torch.Tensor, limit: float = 0.0) -> MXFP4Weights:
     """``silu(gate) * up`` of rows ``[gate | up]`` in MXFP4, [rows, in]; ``limit`` > 0 clamps
     ``gate <= limit`` and ``-limit <= up <= limit`` first."""
+    if gate_up.is_cuda and gate_up.dim() == 2:
+        ctx = Context.get(gate_up.get_device())
+        r = L.load_torch().quantize_swiglu(ctx.address, ctx.device, gate_up, limit)
+        if r is not None:
+            if r.__class__ is int:
+                ctx.check("mr_mxfp4_quantize_swiglu", r)
+            return _weights_of(r[0], r[1], gate_up.shape[0], gate_up.shape[1] // 2, None)
     x, shape, stride = _checked("gate_up", gate_up)
     if len(shape) != 2 or shape[1] % 64 != 0 or shape[1] == 0:
         raise MXFP4BridgeError(
@@ -115,6 +130,14 @@ def _operands(a: MXFP4Weights, w: MXFP4Weights, out_dtype: torch.dtype) -> int:
 def mxfp4_scaled_mm(a: MXFP4Weights, w: MXFP4Weights,
                     out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``a . w^T`` [rows, out] of two MXFP4 matrices, fp32 sums."""
+    if a.experts is None and w.experts is None and out_dtype in _OUT_DTYPES and a.packed.is_cuda:
+        ctx = Context.get(a.packed.get_device())
+        out = L.load_torch().scaled_mm(ctx.address, ctx.device, a.packed, a.scales, w.packed,
+                                       w.scales, out_dtype is torch.float32)
+        if out is not None:
+            if out.__class__ is int:
+                ctx.check("mr_mxfp4_scaled_mm", out)
+            return out
     dt = _operands(a, w, out_dtype)
     if w.experts is not None:
         raise MXFP4BridgeError("mxfp4_scaled_mm needs a single matrix; use mxfp4_grouped_mm")
@@ -135,6 +158,14 @@ def mxfp4_grouped_mm(a: MXFP4Weights, w: MXFP4Weights, plan: SortedTokens,
 
     ``a`` holds the sorted rows, or with ``by_token`` the tokens' rows: row r then takes
     ``a[order[r] // top_k]``, read in place, so a token is quantised once whatever top_k is."""
+    if a.experts is None and w.experts is not None and out_dtype in _OUT_DTYPES:
+        ctx = Context.get(plan.index)
+        out = L.load_torch().grouped_mm(ctx.address, plan.index, a.packed, a.scales, w.packed,
+                                        w.scales, out_dtype is torch.float32, plan._at, by_token)
+        if out is not None:
+            if out.__class__ is int:
+                ctx.check("mr_mxfp4_grouped_mm", out)
+            return out
     dt = _operands(a, w, out_dtype)
     if w.experts is None:
         raise MXFP4BridgeError("mxfp4_grouped_mm needs an expert stack; use mxfp4_scaled_mm")

@@ -51,9 +51,9 @@ class SortedTokens:
     def _fill(self, order, inverse, offsets, tokens, top_k, experts, device):
         self.tokens, self.top_k, self.experts = tokens, top_k, experts
         self.rows = tokens * top_k
-        self.device = device
+        self.device, self.index = device, device.index
         self._c = L.mr_sorted(order, inverse, offsets, tokens, top_k, experts)
-        self._ref = C.byref(self._c)
+        self._ref, self._at = C.byref(self._c), C.addressof(self._c)
 
     @classmethod
     def _of(cls, mem: torch.Tensor, tokens: int, top_k: int, experts: int) -> "SortedTokens":
@@ -66,10 +66,7 @@ class SortedTokens:
 
     def _split(self):
         if self._views is None:
-            P, k = self.rows, self.top_k
-            m = self._mem
-            self._views = (m.as_strided((P,), (1,), 0), m.as_strided((self.tokens, k), (k, 1), P),
-                           m.as_strided((self.experts + 1,), (1,), 2 * P))
+            self._views = L.load_torch().views(self._mem, self.tokens, self.top_k, self.experts)
         return self._views
 
     @property
@@ -87,6 +84,14 @@ class SortedTokens:
 
 def moe_sort(ids: torch.Tensor, experts: int) -> SortedTokens:
     """The pairs of ``ids`` [tokens, top_k] in the order of their experts, stable."""
+    if ids.is_cuda and ids.dim() == 2:
+        ctx = Context.get(ids.get_device())
+        mem = L.load_torch().sort(ctx.address, ctx.device, ids, experts)
+        if mem is not None:
+            if mem.__class__ is int:
+                ctx.check("mr_moe_sort", mem)
+            T, k = ids.shape
+            return SortedTokens._of(mem, T, k, experts)
     if ids.dim() != 2 or not ids.is_cuda:
         raise AffineBridgeError("ids must be a CUDA [tokens, top_k] tensor")
     if ids.dtype != torch.int32:
@@ -133,7 +138,19 @@ def _weights(w: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     return w if w.is_contiguous() else w.contiguous()
 
 
+def _fast(name: str, plan: SortedTokens, *args):
+    """The call by its short way, or None where the tensors are not the plain case."""
+    ctx = Context.get(plan.index)
+    r = getattr(L.load_torch(), name)(ctx.address, plan.index, *args, plan._at)
+    if r.__class__ is int:
+        ctx.check("mr_moe_" + name, r)
+    return r
+
+
 def _dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
+    xs = _fast("dispatch", plan, x)
+    if xs is not None:
+        return xs
     x, H, stride = _rows("x", x, plan.tokens, plan)
     xs = x.new_empty((plan.rows, H))
     ctx = Context.get(plan.device.index)
@@ -146,6 +163,9 @@ def _dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
 
 def moe_dispatch_backward(dxs: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     """Gradient of ``moe_dispatch``: ``dx[t] = sum_j dxs[inverse[t, j]]``, fp32 sums."""
+    dx = _fast("dispatch_backward", plan, dxs)
+    if dx is not None:
+        return dx
     dxs, H, stride = _rows("dxs", dxs, plan.rows, plan)
     dx = dxs.new_empty((plan.tokens, H))
     ctx = Context.get(plan.device.index)
@@ -158,6 +178,10 @@ def moe_dispatch_backward(dxs: torch.Tensor, plan: SortedTokens) -> torch.Tensor
 
 
 def _combine(ys, weights, plan, base) -> torch.Tensor:
+    if base is None:
+        out = _fast("combine", plan, ys, weights)
+        if out is not None:
+            return out
     ys, H, stride = _rows("ys", ys, plan.rows, plan)
     weights = _weights(weights, plan)
     at = None
@@ -181,6 +205,9 @@ def _combine(ys, weights, plan, base) -> torch.Tensor:
 def moe_combine_backward(dout: torch.Tensor, ys: torch.Tensor, weights: torch.Tensor,
                          plan: SortedTokens) -> tuple[torch.Tensor, torch.Tensor]:
     """Gradients ``(dys, dweights)`` of ``moe_combine``; that of ``base`` is ``dout``."""
+    both = _fast("combine_backward", plan, dout, ys, weights)
+    if both is not None:
+        return both
     ys, H, stride = _rows("ys", ys, plan.rows, plan)
     dout, Hd, dstride = _rows("dout", dout, plan.tokens, plan)
     if dout.dtype != ys.dtype or Hd != H:

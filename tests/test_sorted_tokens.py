@@ -62,3 +62,37 @@ def test_sorted_struct_matches_the_c_compiler(tmp_path):
                    check=True)
     got = list(map(int, subprocess.check_output([str(exe)]).split()))
     assert got == [C.sizeof(L.mr_sorted)] + [getattr(L.mr_sorted, n).offset for n in names]
+
+
+def test_short_way_takes_only_the_plain_case():
+    """csrc/mr_torch.cpp answers None for what it leaves to the Python functions: CPU tensors,
+    other types, a wrong number of arguments."""
+    ext = L.load_torch()
+    ids = torch.zeros((4, 2), dtype=torch.int32)
+    x = torch.zeros((4, 64))
+    plan = L.mr_sorted(16, 16, 16, 4, 2, 3)
+    at = C.addressof(plan)
+    w = torch.zeros((4, 2))
+    p, s = torch.zeros((4, 8), dtype=torch.int32), torch.zeros((4, 2), dtype=torch.uint8)
+    assert ext.sort(0, 0, ids, 3) is None
+    assert ext.sort(0, 0, ids) is None
+    assert ext.sort(0, 0, "ids", 3) is None
+    assert ext.dispatch(0, 0, x, at) is None
+    assert ext.dispatch_backward(0, 0, x, at) is None
+    assert ext.combine(0, 0, x, w, at) is None
+    assert ext.combine_backward(0, 0, x, x, w, at) is None
+    assert ext.quantize(0, 0, x, False) is None
+    assert ext.quantize_swiglu(0, 0, x, 0.0) is None
+    assert ext.scaled_mm(0, 0, p, s, p, s, False) is None
+    assert ext.grouped_mm(0, 0, p, s, p, s, False, at, False) is None
+    with pytest.raises(TypeError):
+        ext.bind(1, 2)
+
+
+def test_short_way_binds_every_function_in_order():
+    import os
+    import re
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = open(os.path.join(root, "minirun-app_b200", "csrc", "mr_torch.cpp")).read()
+    names = re.findall(r"decltype\(&(mr_\w+)\)", src)
+    assert tuple(names) == L._TORCH_API

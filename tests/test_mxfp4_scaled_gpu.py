@@ -244,6 +244,13 @@ def test_grouped_mm(T, k, E, out, inn, dropped, by_token):
 
 
 @pytest.mark.parametrize("by_token", [False, True])
+@pytest.mark.parametrize("T", [10, 20, 43, 85, 150])
+def test_grouped_mm_every_tile_width(T, by_token):
+    """Mean rows of 5 to 75 an expert: every width of a tile, over drawn and dropped rows."""
+    grouped(T, 4, 8, 328, 1056, by_token, seed=T, dropped=0.05)
+
+
+@pytest.mark.parametrize("by_token", [False, True])
 def test_grouped_mm_uneven_experts(by_token):
     """One expert with nearly all rows (several tiles), some with one, some with none."""
     ids = np.zeros((900, 1), np.int32)

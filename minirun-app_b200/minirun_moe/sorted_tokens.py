@@ -5,7 +5,8 @@ orders the (token, slot) pairs by expert, ``moe_dispatch`` copies the tokens'
 rows into that order, the experts work on contiguous rows, and
 ``moe_combine`` brings their rows back, weighted and summed. Both copies have
 their gradients, as functions and through torch's autograd: where an input
-requires a gradient, ``moe_dispatch`` and ``moe_combine`` record it.
+requires a gradient, ``moe_dispatch`` and ``moe_combine`` record it. (Gradients
+of the gradients are not built and raise.)
 
 An id of -1 is a slot without an expert: it takes no expert's row, its sorted
 row comes after all experts' and holds zeros, and the combine adds nothing.
@@ -15,6 +16,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from .bridge import AffineBridgeError, Context, _raw_stream
@@ -232,6 +234,7 @@ class _Dispatch(torch.autograd.Function):
         return _dispatch(x, plan)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dxs):
         return moe_dispatch_backward(dxs, ctx.plan), None
 
@@ -244,6 +247,7 @@ class _Combine(torch.autograd.Function):
         return _combine(ys, weights, plan, base)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         ys, weights = ctx.saved_tensors
         dys = dw = None

@@ -202,6 +202,16 @@ def test_autograd_matches_the_functions():
     assert torch.equal(x.grad, M.moe_dispatch_backward(dys, p))
 
 
+def test_gradients_of_gradients_raise():
+    p = M.moe_sort(torch.from_numpy(choice(6, 2, 4, 3)).to(dev()), 4)
+    x = rows(6, 32, torch.float32, 1).requires_grad_()
+    w = torch.full((6, 2), 0.5, device=dev(), requires_grad=True)
+    (dx,) = torch.autograd.grad((M.moe_combine(M.moe_dispatch(x, p), w, p) ** 2).sum(), x,
+                                create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
 def test_strided_rows_match_contiguous_ones():
     """Rows that are slices of wider ones, at every alignment of the row."""
     T, k, E = 19, 2, 5

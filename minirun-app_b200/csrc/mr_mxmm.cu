@@ -110,7 +110,7 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
     return fail(ctx, MR_ERR_UNSUPPORTED, "the product has more than 2^31 tiles");
   p.ksplit = 1;
   // CTAs share a tile where there are few, the rows are long and the tile is
-  // narrow (1 and 16 rows x 2048 x 7168: 8.2 -> 6.2 us and 8.1 -> 6.8; with 32
+  // narrow (1 and 16 rows x 2048 x 7168 in L2: 8.2 -> 6.2 us and 8.1 -> 6.8; with 32
   // rows, or rows of 2048, the exchange costs what the shorter loop saves).
   while (p.ntile == 16 && p.ksplit < kMmSplit && 2 * p.ksplit * tiles <= sms && p.nstages >= 8)
     p.ksplit *= 2;

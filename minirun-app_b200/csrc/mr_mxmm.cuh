@@ -11,8 +11,21 @@
 //
 // CG = 1: one CTA a tile. CG = 2: a cluster of two CTAs a tile of 256 weight
 // rows; each loads its own 128 rows and half of the activations, and the
-// leader's MMAs (cta_group::2) read both halves: per MMA a CTA takes 28 KB
-// from L2 instead of 40.
+// leader's MMAs (cta_group::2) read both halves: per stage of 176 rows a CTA
+// takes 54 KB of codes from L2 instead of 76. That is what bounds a large
+// product: an SM takes 64 bytes a cycle from L2, so a stage of n rows is
+// 512 + 2n cycles of loads (512 + 4n without the pair) against 4n of MMAs.
+//
+// Measured, out bf16: 4096 x 16384 x 7168 209 us (4.6 PFLOP/s); 64 tokens x 8
+// of 256 experts of 2048 x 7168 256 us (0.99 of the copy rate, the weights);
+// one token x 8 of them 14.7 us (floor 9.5): the first copy starts 2.8 us after
+// the kernel does (the table 1.3, the rest the fetch of each role's code), the
+// last tile's result leaves 1.1 us after its codes are there, and between the
+// two HBM runs at 0.99. One row x 2048 x 7168 7.4 us, 6.3 with the weights in
+// L2. (Tried for the start, each within 1 % or slower: the first weights'
+// copies right behind the table, 10.2 -> 11.1 us at 64 experts of 1024 x 4096;
+// the table's code run once on nothing before the wait for the kernels ahead;
+// one tile lookup that every role calls.)
 //
 // Where there are few narrow tiles (CG = 1), a cluster of `ksplit` CTAs shares each:
 // every CTA multiplies its part of the row's stages and leaves the partial
@@ -37,7 +50,7 @@
 //   - warp 1: one MMA per 64 elements. Its lane, like those that issue TMA,
 //     is chosen by elect.sync: from a branch on the lane's number each such
 //     instruction cost 90-110 cycles (its operands live in uniform
-//     registers), so 40; the other lanes leave;
+//     registers), so 30-40; the other lanes leave;
 //   - warps 4-7: a finished tile's accumulator to global memory while the
 //     next tile's MMAs run (two accumulators).
 // Every ring slot has exponents' columns of its own in TMEM, so they are only
@@ -417,7 +430,7 @@ struct MmScaleRegs {
   }
 };
 
-// Exponents from global to shared memory, loaded one or two stages (also of
+// Exponents from global to shared memory, loaded one to four stages (also of
 // the next tile) ahead of their use: the loads' latency stays out of the
 // pipeline. A slot holds 16 bytes a row. Every lane of the warp.
 template <int NB, bool WIDE, bool IS_A, int CG>
@@ -445,7 +458,10 @@ MR_DEVICE void mm_load_scales(const MmParams& p, const MmWalk<CG>& walk, int lan
       src[i] = lo + row * p.groups;
     }
   };
-  constexpr int kAhead = WIDE ? 2 : 1;  // registers of two unaligned stages would spill
+  // Narrow tiles are few stages of HBM's latency long: four ahead against two is
+  // 15.3 -> 14.7 us for a token's 8 experts of 2048 x 7168. Wide ones load from
+  // L2 and lose 1 % by it. Registers of two unaligned stages would spill.
+  constexpr int kAhead = !WIDE ? 1 : CG == 1 ? 4 : 2;
   MmScaleRegs<NB, WIDE> v[kAhead];
 #pragma unroll
   for (int b = 0; b < kAhead; ++b)

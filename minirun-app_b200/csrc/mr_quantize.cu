@@ -141,7 +141,11 @@ MR_DEVICE void quantize8(const QuantParams& p, int64_t o, const float (&f)[8]) {
   }
 }
 
-// U octets a thread, a CTA apart, all loads first.
+// Four lanes a block of 32: one 16-byte load (two of fp32) and one word of codes
+// a lane, the block's maximum by two shuffles. U octets a thread, a CTA apart,
+// all loads first. Bound by HBM: fp32 16384 x 7168 with the values back 150 us
+// (the copy rate); bf16 8192 x 2048 with SwiGLU 15 us (floor 12); bf16 64 x 7168
+// 1.9 us, a launch.
 template <int DT, bool ALIGNED, bool SWIGLU, int U>
 __global__ void __launch_bounds__(kQThreads) quantize_kernel(const QuantParams p) {
   constexpr int kOct = DT == MR_DTYPE_F32 ? 32 : 16;  // bytes of an octet

@@ -55,6 +55,9 @@
 //     next tile's MMAs run (two accumulators).
 // Every ring slot has exponents' columns of its own in TMEM, so they are only
 // overwritten once the MMAs that read them are complete.
+// Tensor-memory loads, stores and (de)allocation are warp-aligned: each is
+// preceded by __syncwarp wherever the lanes may have parted (waits, stores of
+// a row's last weight rows).
 // Every wait is bounded: on expiry the kernel flags MR_DEVERR_TIMEOUT and
 // runs to its end on garbage, drains its copies and MMAs, frees its TMEM.
 #pragma once
@@ -755,6 +758,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
           rphase ^= 1u;
         }
         wait_mbar(empty + slot, phase ^ 1u, flags, p.error, free);
+        __syncwarp();  // lanes may leave a wait one by one
         tc_fence_after();
         // columns 4 w + i (B: sfw w + i): word w of rows lane + 32 i
         const uint32_t t = lane_t + slot * sfc;
@@ -828,6 +832,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       it.at(item);
       const uint32_t db = t & 1u;
       wait_mbar(dfull + db, (t >> 1) & 1u, flags, p.error);
+      __syncwarp();
       tc_fence_after();
       const int64_t o = it.m0 + q * 32 + lane;
       const uint32_t d_t = tbase + db * p.ntile + ((uint32_t)(q * 32) << 16);
@@ -836,6 +841,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         wait_mbar(pempty, (t & 1u) ^ 1u, flags, p.error);
         for (int c = 0; c < it.n; c += 16) {
           float v[16];
+          __syncwarp();
           tmem_ld16(d_t + c, v);
 #pragma unroll
           for (int i = 0; i < 16; ++i) part[(c + i) * kMmRows + row] = v[i];
@@ -886,13 +892,14 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       }
       for (int c = 0; c < it.n; c += 16) {
         float v[16];
+        __syncwarp();  // the lanes' stores below may differ
         tmem_ld16(d_t + c, v);
-        if (o >= p.out_features) continue;
+        const int left = o < p.out_features ? it.n - c : 0;
         const int64_t at = ((int64_t)it.row0 + c) * p.out_features + o;
         if (p.out_f32)
-          store16(reinterpret_cast<float*>(p.out) + at, p.out_features, it.n - c, v);
+          store16(reinterpret_cast<float*>(p.out) + at, p.out_features, left, v);
         else
-          store16(reinterpret_cast<uint16_t*>(p.out) + at, p.out_features, it.n - c, v);
+          store16(reinterpret_cast<uint16_t*>(p.out) + at, p.out_features, left, v);
       }
       tc_fence_before();
       __syncwarp();
@@ -913,6 +920,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         for (int s = 0; s < nst && (uint32_t)s <= last; ++s)
           wait_mbar(empty + s, ((uint32_t)s <= r ? a : a - 1) & 1u, flags, p.error);
       }
+      __syncwarp();
       tc_fence_after();
       mm_tmem_dealloc<CG>();
       if constexpr (CG == 2) {

@@ -1,0 +1,54 @@
+"""MXFP4 x MXFP4 products at the sizes of tiles, on the GPU, against fp64.
+
+The bound is that of a sum of exact products over in/64 tensor-core steps, each
+within 2^-22 of the magnitudes it adds; rounding to bf16 adds half an ulp, 2^-8.
+"""
+import numpy as np
+import pytest
+import torch
+
+import minirun_moe as M
+
+pytestmark = pytest.mark.gpu
+
+GRID = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def dev():
+    return torch.device("cuda", 0)
+
+
+def matrix(rows, width, seed, experts=None):
+    g = torch.Generator(device=dev()).manual_seed(seed)
+    lead = (experts, rows) if experts else (rows,)
+    packed = torch.randint(0, 2 ** 32, lead + (width // 8,), generator=g, device=dev())
+    scales = torch.randint(120, 127, lead + (width // 32,), generator=g, device=dev())
+    return M.MXFP4Weights((packed - 2 ** 31).to(torch.int32), scales.to(torch.uint8))
+
+
+def values(w):
+    """The numbers of a matrix or a stack, fp64."""
+    lut = torch.tensor(GRID + tuple(-v for v in GRID), dtype=torch.float64, device=dev())
+    word = w.packed.long().unsqueeze(-1) >> torch.arange(0, 32, 4, device=dev())
+    scale = ((w.scales.long() + (1023 - 127)) << 52).view(torch.float64)
+    return lut[(word & 15).flatten(-2)] * scale.repeat_interleave(32, dim=-1)
+
+
+def check(got, ref, mag, width):
+    tol = (width / 64 + 2) * 2.0 ** -22 * mag
+    if got.dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * (ref.abs() + tol)
+    over = (got.double() - ref).abs() - tol
+    assert bool((over <= 0).all()), float(over.max())
+    assert M.Context.get(0).sync_check() == 0
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [33, 64, 100, 177])  # one CTA a tile, and two
+@pytest.mark.parametrize("out,width", [(1, 512), (136, 512), (250, 544), (303, 1024), (33, 96)])
+def test_rows_of_weights_that_end_inside_a_warp(rows, out, width, out_dtype):
+    """Several groups of 16 result rows where some lanes of a warp have no weight row."""
+    a, w = matrix(rows, width, rows), matrix(out, width, out)
+    A, W = values(a), values(w)
+    y = M.mxfp4_scaled_mm(a, w, out_dtype=out_dtype)
+    check(y, A @ W.T, A.abs() @ W.abs().T, width)

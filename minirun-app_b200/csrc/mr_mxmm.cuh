@@ -59,7 +59,9 @@
 // preceded by __syncwarp wherever the lanes may have parted (waits, stores of
 // a row's last weight rows).
 // Every wait is bounded: on expiry the kernel flags MR_DEVERR_TIMEOUT and
-// runs to its end on garbage, drains its copies and MMAs, frees its TMEM.
+// runs to its end on garbage, drains its copies and MMAs, frees its TMEM. No
+// CTA of a cluster leaves before every thread of the others is done with its
+// memory (leave_cluster), also where one of them gave up a wait early.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -265,6 +267,15 @@ MR_DEVICE void arrive_all(uint64_t* bar, int ctas) {
         "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [r]; }" ::"r"(smem_u32(bar)),
         "r"(c)
         : "memory");
+}
+
+// The last thing a thread of a cluster of CTAs does: what it did to another
+// CTA's memory is done, and it waits for all threads of the cluster that have
+// not ended to say the same. (The CTAs' own barriers cannot serve for this: a
+// CTA whose wait expired leaves its further waits early.)
+MR_DEVICE void leave_cluster() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // wait_bounded as one look at the barrier and a call where that is not
@@ -534,8 +545,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
   uint64_t* dempty = dfull + 2;       // [2]
   uint64_t* drain = dempty + 2;       // every MMA complete
   uint64_t* done = drain + 1;         // every other access of TMEM too
-  uint64_t* bye = done + 1;           // the other CTA needs this one's memory no more
-  uint64_t* pfull = bye + 1;          // every CTA's partial result is there (ksplit > 1)
+  uint64_t* pfull = done + 1;         // every CTA's partial result is there (ksplit > 1)
   uint64_t* pempty = pfull + 1;       // this CTA's has been read by all
   uint32_t* tslot = reinterpret_cast<uint32_t*>(pempty + 1);
   volatile int* flags = reinterpret_cast<volatile int*>(tslot + 1);
@@ -569,7 +579,6 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     }
     mbar_init(drain, 1);
     mbar_init(done, rank == 0 ? 8 : 9);
-    mbar_init(bye, 1);
     mbar_init(pfull, 4 * ks);
     mbar_init(pempty, 4 * ks);
     flags[0] = 0;
@@ -685,6 +694,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
           }
         }
       mbar_arrive(done);
+      leave_cluster();
       return;
     }
     const int sfc = mm_sf_cols(p.ntile), sfw = mm_sf_word(p.ntile);
@@ -905,8 +915,6 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       __syncwarp();
       if (lane == 0) mm_arrive<CG>(dempty + db, 0, rank);
     }
-    // every CTA has read this one's last partial result
-    if (ks > 1 && t > 0) wait_mbar(pempty, (t - 1) & 1u, flags, p.error);
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(done);
@@ -923,12 +931,6 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       __syncwarp();
       tc_fence_after();
       mm_tmem_dealloc<CG>();
-      if constexpr (CG == 2) {
-        // this CTA's arrivals at the other are all made, and the MMAs that
-        // read this one's memory done: leave when the other says the same
-        if (lane == 0) mm_arrive<CG>(bye, rank ^ 1u, rank);
-        wait_mbar(bye, 0, flags, p.error);
-      }
     }
     // rows without a pair
     const int64_t z0 = (int64_t)goff[p.E] * p.out_features, z1 = p.rows * p.out_features;
@@ -940,6 +942,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         reinterpret_cast<uint16_t*>(p.out)[i] = 0;
     }
   }
+  if (CG * ks > 1) leave_cluster();
 }
 
 }  // namespace mr

@@ -52,3 +52,47 @@ def test_rows_of_weights_that_end_inside_a_warp(rows, out, width, out_dtype):
     A, W = values(a), values(w)
     y = M.mxfp4_scaled_mm(a, w, out_dtype=out_dtype)
     check(y, A @ W.T, A.abs() @ W.abs().T, width)
+
+
+def sorted_rows(counts, top_k, seed, dropped=0):
+    """A plan whose experts have these numbers of pairs, in random order, `dropped` slots more."""
+    ids = np.concatenate([np.repeat(np.arange(len(counts)), counts), np.full(dropped, -1)])
+    ids = np.concatenate([ids, np.full(-len(ids) % top_k, -1)]).astype(np.int32)
+    ids = np.random.default_rng(seed).permutation(ids).reshape(-1, top_k)
+    return M.moe_sort(torch.from_numpy(ids).to(dev()), len(counts))
+
+
+def check_grouped(counts, out, width, by_token, seed, out_dtype=torch.bfloat16, top_k=2,
+                  dropped=0):
+    p = sorted_rows(counts, top_k, seed, dropped)
+    a = matrix(p.tokens if by_token else p.rows, width, seed + 1)
+    w = matrix(out, width, seed + 2, experts=len(counts))
+    got = M.mxfp4_grouped_mm(a, w, p, by_token=by_token, out_dtype=out_dtype)
+    A = values(a)
+    ref = torch.zeros((p.rows, out), dtype=torch.float64, device=dev())
+    mag = torch.zeros_like(ref)
+    off, order = p.offsets.tolist(), p.order.long()
+    for e in range(len(counts)):
+        r = slice(off[e], off[e + 1])
+        x = A[order[r] // top_k] if by_token else A[r]
+        W = values(M.MXFP4Weights(w.packed[e], w.scales[e]))
+        ref[r], mag[r] = x @ W.T, x.abs() @ W.abs().T
+    check(got, ref, mag, width)
+    return a, w, p, got
+
+
+@pytest.mark.parametrize("by_token", [False, True])
+@pytest.mark.parametrize("counts,out,width", [
+    ([3, 0, 1], 256, 4096),           # four CTAs a tile
+    ([0, 0, 0], 256, 4096),           # and none of them with one
+    ([150, 90, 0, 200], 600, 1024),   # two CTAs a tile
+    ([0, 0, 0, 0], 600, 1024),
+])
+def test_clusters_end_together(counts, out, width, by_token):
+    """Tiles shared by a cluster's CTAs, call after call, with rows that no expert takes: always
+    the same results."""
+    a, w, p, first = check_grouped(counts, out, width, by_token, 7, dropped=400 if out == 600
+                                   else 5)
+    for _ in range(20):
+        assert torch.equal(first, M.mxfp4_grouped_mm(a, w, p, by_token=by_token))
+    assert bool((first[sum(counts):] == 0).all())

@@ -550,6 +550,9 @@ mr_status check_plan(mr_ctx* ctx, const mr_sorted* s) {
     return fail(ctx, MR_ERR_UNSUPPORTED, "more than 2^31 - 1 (token, slot) pairs");
   if (!s->offsets || (s->tokens > 0 && (!s->order || !s->inverse)))
     return fail(ctx, MR_ERR_INVALID_ARGUMENT, "order, inverse and offsets must be non-NULL");
+  if ((addr(s->order) | addr(s->inverse) | addr(s->offsets)) % 4)
+    return fail(ctx, MR_ERR_INVALID_ARGUMENT,
+                "order, inverse and offsets must be aligned to their type");
   return MR_OK;
 }
 
@@ -679,6 +682,8 @@ mr_status mr_moe_sort(mr_ctx* ctx, const int32_t* ids, int64_t tokens, int32_t t
     const mr_sorted s{order, inverse, offsets, tokens, top_k, experts};
     if (mr_status st = check_plan(ctx, &s)) return st;
     if (tokens > 0 && !ids) return fail(ctx, MR_ERR_INVALID_ARGUMENT, "ids must be non-NULL");
+    if (addr(ids) % 4)
+      return fail(ctx, MR_ERR_INVALID_ARGUMENT, "ids must be aligned to their type");
     if (experts > kMaxExperts)
       return fail(ctx, MR_ERR_UNSUPPORTED, "expert counts above 1024 are not built here");
     SortParams p{ids, tokens * top_k, experts, 0, 0, order, inverse, offsets, ctx->d_error};
@@ -767,6 +772,8 @@ mr_status mr_moe_combine(mr_ctx* ctx, const void* ys, mr_dtype dtype, int64_t ys
     if (mr_status st = check_rows(ctx, plan, dtype, hidden, {ys, out}, {ys_stride})) return st;
     if (plan->tokens == 0) return MR_OK;
     if (!weights) return fail(ctx, MR_ERR_INVALID_ARGUMENT, "weights must be non-NULL");
+    if (addr(weights) % 4)
+      return fail(ctx, MR_ERR_INVALID_ARGUMENT, "weights must be aligned to their type");
     if (addr(base) % elem_bytes(dtype))
       return fail(ctx, MR_ERR_INVALID_ARGUMENT, "row buffers must be aligned to their type");
     return combine_rows(ctx, ys, dtype, ys_stride, hidden, weights, base, plan, out, stream,
@@ -786,6 +793,9 @@ mr_status mr_moe_combine_backward(mr_ctx* ctx, const void* dout, int64_t dout_st
     if (plan->tokens == 0) return MR_OK;
     if (!weights || !dweights)
       return fail(ctx, MR_ERR_INVALID_ARGUMENT, "weights and dweights must be non-NULL");
+    if ((addr(weights) | addr(dweights)) % 4)
+      return fail(ctx, MR_ERR_INVALID_ARGUMENT,
+                  "weights and dweights must be aligned to their type");
     const int es = elem_bytes(dtype);
     const int vb = vec_bytes({addr(dout), addr(ys), addr(dys), (uint64_t)(dout_stride * es),
                               (uint64_t)(ys_stride * es), (uint64_t)(hidden * es)});

@@ -1,10 +1,13 @@
 """Sorted tokens at the sizes that choose a kernel's form, on the GPU, against
 the formulas in numpy and fp64."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
 import minirun_moe as M
+from minirun_moe import _lib as L
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +47,43 @@ def test_sort_where_experts_end_inside_a_warp(T, k, E, dropped):
     np.testing.assert_array_equal(p.inverse.cpu().numpy(), inverse)
     np.testing.assert_array_equal(p.offsets.cpu().numpy(), offsets)
     assert M.Context.get(0).sync_check() == 0
+
+
+def test_misaligned_pointers_are_refused():
+    """Every int32 and fp32 pointer of the C entries two bytes off its alignment: refused before a
+    launch."""
+    T, k, E, H = 4, 2, 3, 64
+    lib, ctx = L.load(), M.Context.get(0)
+    ids = torch.zeros((T, k), dtype=torch.int32, device=dev())
+    p = M.moe_sort(ids, E)
+    x, ys = torch.zeros((T, H), device=dev()), torch.zeros((T * k, H), device=dev())
+    w = torch.zeros((T, k), device=dev())
+    mem = torch.zeros(2 * T * k + E + 1, dtype=torch.int32, device=dev())
+    i, o = ids.data_ptr(), mem.data_ptr()
+    n, f = o + 4 * T * k, o + 8 * T * k
+    s = torch.cuda.current_stream().cuda_stream
+
+    def refused(st):
+        assert st == L.MR_ERR_INVALID_ARGUMENT
+        assert b"aligned" in lib.mr_last_error(ctx.handle)
+
+    for at in range(4):
+        a = [q + 2 * (at == j) for j, q in enumerate((i, o, n, f))]
+        refused(lib.mr_moe_sort(ctx.handle, a[0], T, k, E, a[1], a[2], a[3], s))
+    for name in ("order", "inverse", "offsets"):
+        c = L.mr_sorted.from_buffer_copy(p._c)
+        setattr(c, name, getattr(c, name) + 2)
+        ref = C.byref(c)
+        X, Y, W, F = x.data_ptr(), ys.data_ptr(), w.data_ptr(), L.MR_DTYPE_F32
+        refused(lib.mr_moe_dispatch(ctx.handle, X, F, H, H, ref, Y, s))
+        refused(lib.mr_moe_dispatch_backward(ctx.handle, Y, F, H, H, ref, X, s))
+        refused(lib.mr_moe_combine(ctx.handle, Y, F, H, H, W, None, ref, X, s))
+        refused(lib.mr_moe_combine_backward(ctx.handle, X, H, Y, H, F, H, W, ref, Y, W, s))
+        q = M.mxfp4_quantize(x)
+        stack = M.mxfp4_quantize(torch.zeros((E, 32, H), device=dev()))
+        refused(lib.mr_mxfp4_grouped_mm(ctx.handle, C.byref(q.desc()), C.byref(stack.desc()), ref,
+                                        1, F, Y, s))
+    ref = C.byref(p._c)
+    refused(lib.mr_moe_combine(ctx.handle, Y, F, H, H, W + 2, None, ref, X, s))
+    for a, b in ((2, 0), (0, 2)):
+        refused(lib.mr_moe_combine_backward(ctx.handle, X, H, Y, H, F, H, W + a, ref, Y, W + b, s))

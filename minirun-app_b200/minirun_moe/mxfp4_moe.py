@@ -28,7 +28,7 @@ from .sorted_tokens import moe_combine, moe_sort
 class MXFP4MoELayer:
     """``gate_up``: MXFP4 stack [E, 2 * inter, hidden], gate rows first; ``down``: [E, hidden,
     inter]; ``shared``: (gate_up [2 * shared_inter, hidden], down [hidden, shared_inter]) or
-    None; ``router_w`` bf16 [E, hidden]."""
+    None; ``router_w`` bf16 [E, hidden]. All on one GPU, which need not be the current one."""
 
     def __init__(self, router_w: torch.Tensor, gate_up: MXFP4Weights, down: MXFP4Weights,
                  router: RouterConfig,
@@ -50,6 +50,12 @@ class MXFP4MoELayer:
                                     "[2 * shared_inter, hidden] and [hidden, shared_inter]")
         if swiglu_limit < 0:
             raise AffineBridgeError("SwiGLU limit must be >= 0 (0: off)")
+        mats = (gate_up, down, *(shared or ()))
+        devices = {router_w.device, *(t.device for m in mats for t in (m.packed, m.scales))}
+        if len(devices) > 1:
+            raise AffineBridgeError("router and expert weights must be on one device, got "
+                                    + ", ".join(sorted(map(str, devices))))
+        self.device = router_w.device
         self.router_w = router_w.contiguous()
         self.gate_up, self.down, self.router, self.shared = gate_up, down, router, shared
         self.swiglu_limit = float(swiglu_limit)
@@ -74,6 +80,15 @@ class MXFP4MoELayer:
             raise AffineBridgeError(
                 f"input must be a [tokens, {self.hidden}] bfloat16 matrix, got {list(x.shape)} "
                 f"{x.dtype}")
+        if x.device != self.device:
+            raise AffineBridgeError(f"input is on {x.device}, the layer on {self.device}")
+        if x.is_cuda and x.device.index != torch.cuda.current_device():
+            # the router launches on the current device and its stream, the rest on x's
+            with torch.cuda.device(x.device):
+                return self._forward(x)
+        return self._forward(x)
+
+    def _forward(self, x: torch.Tensor) -> tuple[torch.Tensor, Selection]:
         sel = router_select(x, self.router_w, self.router)
         plan = moe_sort(sel.ids, self.router.experts)
         xq = mxfp4_quantize(x)

@@ -241,7 +241,7 @@ mr_status mr_mxfp4_dequantize(mr_ctx* ctx, const mr_mxfp4_desc* w, float* out,
 mr_status mr_mxfp4_quantize(mr_ctx* ctx, const void* x, mr_dtype dtype, int64_t rows,
                             int64_t in_features, int64_t x_stride, uint32_t* packed,
                             uint8_t* scales, void* values, void* stream);
-/* The same of h = silu(gate) * up (fp32), for gate_up rows [gate | up] of
+/* The same of h = silu(gate) * up (fp32, within 2^-20), for gate_up rows [gate | up] of
  * 2 * inter elements, stride elements apart: what the second expert product
  * takes, without h in memory. swiglu_limit > 0: gate <= L, -L <= up <= L. */
 mr_status mr_mxfp4_quantize_swiglu(mr_ctx* ctx, const void* gate_up, mr_dtype dtype, int64_t rows,

@@ -141,6 +141,41 @@ MR_DEVICE void quantize8(const QuantParams& p, int64_t o, const float (&f)[8]) {
   }
 }
 
+// silu(gate) * up for any gate. Far below zero 1 + exp(-gate) overflows and
+// 1 + exp(gate) is 1: gate * exp(gate / 2) * up * exp(gate / 2), of which no step
+// leaves fp32's range before the result does. CUDA's expf is within 2 ulp.
+MR_DEVICE float silu_times(float gate, float up) {
+  if (gate < -80.f) {
+    const float e = expf(0.5f * gate);
+    return gate * e * up * e;
+  }
+  return gate / (1.f + expf(-gate)) * up;
+}
+// f = silu(f) * g of eight. For gates of 80 units at most exp(-f) is 2^t with t =
+// -f log2(e) rounded, times 1 + r for what the rounding left, r = -f - t ln(2) (a
+// residual as in Cody and Waite's reductions): with ex2.approx and __fdividef,
+// 2 ulp each, all of it is within 2^-20. Taking exp2(t) alone, as __expf does,
+// loses an ulp for every unit of f; expf for all gates costs 4 us of 19 at 8192
+// x 2048, with an IEEE division 9 of 24.
+MR_DEVICE void silu8(float (&f)[8], const float (&g)[8]) {
+  float most = fabsf(f[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) most = fmaxf(most, fabsf(f[i]));
+  if (most > 80.f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = silu_times(f[i], g[i]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = f[i] * -1.44269504088896341f;
+    const float r = fmaf(t, -0.693147180559945309f, -f[i]);
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    f[i] = __fdividef(f[i], 1.f + fmaf(e, r, e)) * g[i];
+  }
+}
+
 // Four lanes a block of 32: one 16-byte load (two of fp32) and one word of codes
 // a lane, the block's maximum by two shuffles. U octets a thread, a CTA apart,
 // all loads first. Bound by HBM: fp32 16384 x 7168 with the values back 150 us
@@ -167,18 +202,16 @@ __global__ void __launch_bounds__(kQThreads) quantize_kernel(const QuantParams p
     if constexpr (SWIGLU) {
       float g[8];
       to_float<DT>(b[u], g);
+      if (p.limit > 0.f) {
+        // comparisons, not fmin/fmax: a NaN stays one
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float gate = f[i], up = g[i];
-        if (p.limit > 0.f) {
-          // comparisons, not fmin/fmax: a NaN stays one
-          if (gate > p.limit) gate = p.limit;
-          if (up > p.limit) up = p.limit;
-          if (up < -p.limit) up = -p.limit;
+        for (int i = 0; i < 8; ++i) {
+          if (f[i] > p.limit) f[i] = p.limit;
+          if (g[i] > p.limit) g[i] = p.limit;
+          if (g[i] < -p.limit) g[i] = -p.limit;
         }
-        // fast exp and divide: a few ulp of fp32, against the 4-bit rounding
-        f[i] = __fdividef(gate, 1.f + __expf(-gate)) * up;
       }
+      silu8(f, g);
     }
     quantize8<DT>(p, o0 + u * kQThreads, f);
   }

@@ -99,7 +99,8 @@ def moe_sort(ids: torch.Tensor, experts: int) -> SortedTokens:
     if ids.dtype != torch.int32:
         if ids.dtype != torch.int64:
             raise AffineBridgeError(f"ids must be int32 or int64, got {ids.dtype}")
-        ids = ids.to(torch.int32)
+        # an id out of int32's range stays out of range, and -1 the only one without an error
+        ids = ids.clamp(-2, 2 ** 31 - 1).to(torch.int32)
     if not ids.is_contiguous():
         ids = ids.contiguous()
     T, k = ids.shape

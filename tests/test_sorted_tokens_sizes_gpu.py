@@ -87,3 +87,16 @@ def test_misaligned_pointers_are_refused():
     refused(lib.mr_moe_combine(ctx.handle, Y, F, H, H, W + 2, None, ref, X, s))
     for a, b in ((2, 0), (0, 2)):
         refused(lib.mr_moe_combine_backward(ctx.handle, X, H, Y, H, F, H, W + a, ref, Y, W + b, s))
+
+
+@pytest.mark.parametrize("bad", [2 ** 32 + 3, 2 ** 32, 2 ** 31, 2 ** 32 - 1, -2, -2 ** 31 - 1,
+                                 -2 ** 32 - 1, -2 ** 63, 2 ** 63 - 1])
+def test_int64_ids_out_of_range_are_reported_and_dropped(bad):
+    ids = torch.tensor([[0, 3], [bad, 1], [-1, 3]], device=dev())
+    p = M.moe_sort(ids, 4)
+    assert p.inverse.tolist() == [[0, 2], [-1, 1], [-1, 3]]
+    assert p.offsets.tolist() == [0, 1, 2, 2, 4] and p.order.tolist() == [0, 3, 1, 5, -1, -1]
+    with pytest.raises(M.MoeError, match="expert id out of range"):
+        M.Context.get(0).sync_check()
+    M.moe_sort(torch.tensor([[0, -1]], device=dev()), 4)
+    assert M.Context.get(0).sync_check() == 0

@@ -16,6 +16,9 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <exception>
+
 #include "minirun_moe.h"
 
 namespace {
@@ -32,11 +35,15 @@ struct Api {
   decltype(&mr_mxfp4_grouped_mm) grouped_mm;
 } api;
 
+// A Python exception is set already (an argument that is no number or truth value).
+struct Raised : std::exception {};
+
 // A C++ exception (an allocation that failed) becomes a Python one.
 template <typename F>
 PyObject* guarded(F&& f) {
   try {
     return f();
+  } catch (const Raised&) {
   } catch (const c10::OutOfMemoryError& e) {
     PyErr_SetString(PyExc_MemoryError, e.what_without_backtrace());
   } catch (const c10::Error& e) {
@@ -59,7 +66,16 @@ PyObject* pair(at::Tensor a, at::Tensor b) {
 
 struct Args {
   PyObject* const* v;
-  int64_t num(int i) const { return PyLong_AsLongLong(v[i]); }
+  int64_t num(int i) const {
+    const long long n = PyLong_AsLongLong(v[i]);
+    if (n == -1 && PyErr_Occurred()) throw Raised();
+    return n;
+  }
+  bool flag(int i) const {
+    const int b = PyObject_IsTrue(v[i]);
+    if (b < 0) throw Raised();
+    return b != 0;
+  }
   template <typename T>
   T* at(int i) const {
     return static_cast<T*>(PyLong_AsVoidPtr(v[i]));
@@ -116,7 +132,8 @@ FUNC(sort) {
       return none();
     const int64_t T = ids->size(0), k = ids->size(1), P = T * k;
     if (k > INT32_MAX) return none();
-    at::Tensor mem = empty({2 * P + E + 1}, at::kInt, dev);
+    // (more than 1024 experts are refused)
+    at::Tensor mem = empty({2 * P + std::min<int64_t>(E, 1024) + 1}, at::kInt, dev);
     int32_t* m = mem.mutable_data_ptr<int32_t>();
     const mr_status st = api.sort(a.at<mr_ctx>(0), ids->const_data_ptr<int32_t>(), T, (int32_t)k,
                                   (int32_t)E, m, m + P, m + 2 * P, stream_of(dev));
@@ -224,7 +241,7 @@ FUNC(quantize) {
     at::Tensor packed = empty({rows, n / 8}, at::kInt, dev);
     at::Tensor scales = empty({rows, n / 32}, at::kByte, dev);
     at::Tensor values;
-    const bool want = PyObject_IsTrue(argv[3]) == 1;
+    const bool want = a.flag(3);
     if (want) values = empty({rows, n}, x->scalar_type(), dev);
     const mr_status st = api.quantize(
         a.at<mr_ctx>(0), x->const_data_ptr(), dt, rows, n, n,
@@ -293,9 +310,9 @@ FUNC(product) {
         !operand(a.tensor(4, dev), a.tensor(5, dev), GROUPED, &w) ||
         x.in_features != w.in_features)
       return none();
-    const bool f32 = PyObject_IsTrue(argv[6]) == 1;
+    const bool f32 = a.flag(6);
     const mr_sorted* plan = GROUPED ? a.at<mr_sorted>(7) : nullptr;
-    const bool by_token = GROUPED && PyObject_IsTrue(argv[8]) == 1;
+    const bool by_token = GROUPED && a.flag(8);
     int64_t rows = x.out_features;
     if (GROUPED) {
       rows = plan->tokens * plan->top_k;

@@ -103,8 +103,10 @@ def moe_sort(ids: torch.Tensor, experts: int) -> SortedTokens:
         ids = ids.clamp(-2, 2 ** 31 - 1).to(torch.int32)
     if not ids.is_contiguous():
         ids = ids.contiguous()
+    if not -2 ** 31 <= experts < 2 ** 31:
+        raise AffineBridgeError(f"experts must be a number of 32 bits, got {experts}")
     T, k = ids.shape
-    mem = ids.new_empty((2 * T * k + max(experts, 0) + 1,))
+    mem = ids.new_empty((2 * T * k + min(max(experts, 0), 1024) + 1,))  # more are refused
     s = SortedTokens._of(mem, T, k, experts)
     c, ctx = s._c, Context.get(s.device.index)
     st = L.load().mr_moe_sort(ctx.handle, ids.data_ptr(), T, k, experts, c.order, c.inverse,

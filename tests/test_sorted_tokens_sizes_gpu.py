@@ -100,3 +100,25 @@ def test_int64_ids_out_of_range_are_reported_and_dropped(bad):
         M.Context.get(0).sync_check()
     M.moe_sort(torch.tensor([[0, -1]], device=dev()), 4)
     assert M.Context.get(0).sync_check() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_counts_of_experts_that_are_none(dtype):
+    ids = torch.zeros((4, 2), dtype=dtype, device=dev())
+    for experts in (2 ** 32 + 3, 2 ** 31, -2 ** 31 - 1):
+        with pytest.raises(M.AffineBridgeError, match="32 bits"):
+            M.moe_sort(ids, experts)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    for experts in (0, -1, 1025, 2 ** 31 - 1):
+        with pytest.raises(M.MoeError):
+            M.moe_sort(ids, experts)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+    with pytest.raises(TypeError):
+        M.moe_sort(ids, 3.0)
+
+
+def test_a_values_flag_without_a_truth_value():
+    x = torch.zeros((2, 64), device=dev())
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        M.mxfp4_quantize(x, values=torch.zeros(2))

@@ -6,7 +6,8 @@ rows into that order, the experts work on contiguous rows, and
 ``moe_combine`` brings their rows back, weighted and summed. Both copies have
 their gradients, as functions and through torch's autograd: where an input
 requires a gradient, ``moe_dispatch`` and ``moe_combine`` record it. (Gradients
-of the gradients are not built and raise.)
+of the gradients and forward-mode tangents are not built and raise; the gradient
+functions themselves record nothing.)
 
 An id of -1 is a slot without an expert: it takes no expert's row, its sorted
 row comes after all experts' and holds zeros, and the combine adds nothing.
@@ -16,6 +17,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -259,9 +261,22 @@ class _Combine(torch.autograd.Function):
         return dys, dw, None, dout if ctx.needs_input_grad[3] else None
 
 
+def _recorded(*tensors) -> bool:
+    """Whether autograd has a part in the call: a gradient to record, or a tangent, which the
+    autograd functions refuse."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0:
+        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                   for t in tensors)
+    return False
+
+
 def moe_dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     """``xs[r] = x[order[r] // top_k]`` [tokens * top_k, hidden]; rows without a pair are zero."""
-    if x.requires_grad and torch.is_grad_enabled():
+    if _recorded(x):
         return _Dispatch.apply(x, plan)
     return _dispatch(x, plan)
 
@@ -270,7 +285,6 @@ def moe_combine(ys: torch.Tensor, weights: torch.Tensor, plan: SortedTokens,
                 base: torch.Tensor | None = None) -> torch.Tensor:
     """``out[t] = base[t] + sum_j weights[t, j] * ys[inverse[t, j]]``: fp32 sums in slot order,
     one rounding to the type of ``ys``. ``base``: rows to add (the shared expert's)."""
-    if torch.is_grad_enabled() and (ys.requires_grad or weights.requires_grad or
-                                    (base is not None and base.requires_grad)):
+    if _recorded(ys, weights, base):
         return _Combine.apply(ys, weights, plan, base)
     return _combine(ys, weights, plan, base)

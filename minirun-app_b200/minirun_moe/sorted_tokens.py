@@ -48,7 +48,7 @@ class SortedTokens:
                 raise AffineBridgeError("sorted tokens are contiguous CUDA int32 tensors")
             if t.device != order.device:
                 raise AffineBridgeError("sorted tokens must be on one device")
-        self._views = (order, inverse, offsets)
+        self._mem, self._views = None, (order, inverse, offsets)
         self._fill(order.data_ptr(), inverse.data_ptr(), offsets.data_ptr(), inverse.shape[0],
                    inverse.shape[1], experts, order.device)
 
@@ -72,6 +72,12 @@ class SortedTokens:
         if self._views is None:
             self._views = L.load_torch().views(self._mem, self.tokens, self.top_k, self.experts)
         return self._views
+
+    def _version(self) -> tuple:
+        """Tells whether the plan's tensors were written between two calls (in place, by torch; an
+        inference tensor does not count its writes)."""
+        mine = self._views if self._mem is None else (self._mem,)
+        return tuple(-1 if t.is_inference() else t._version for t in mine)
 
     @property
     def order(self) -> torch.Tensor:
@@ -232,28 +238,36 @@ def moe_combine_backward(dout: torch.Tensor, ys: torch.Tensor, weights: torch.Te
     return dys, dw
 
 
+def _unchanged(ctx) -> None:
+    if ctx.plan._version() != ctx.version:
+        raise RuntimeError("the sorted tokens were modified by an inplace operation between "
+                           "forward and backward")
+
+
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
-        ctx.plan = plan
+        ctx.plan, ctx.version = plan, plan._version()
         return _dispatch(x, plan)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dxs):
+        _unchanged(ctx)
         return moe_dispatch_backward(dxs, ctx.plan), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ys, weights, plan, base):
-        ctx.plan = plan
+        ctx.plan, ctx.version = plan, plan._version()
         ctx.save_for_backward(ys, weights)
         return _combine(ys, weights, plan, base)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        _unchanged(ctx)
         ys, weights = ctx.saved_tensors
         dys = dw = None
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:

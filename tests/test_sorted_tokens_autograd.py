@@ -56,3 +56,35 @@ def test_forward_mode_raises(plan, grad_mode):
                 f()
         # tensors without a tangent go as ever
         assert M.moe_combine(M.moe_dispatch(x, plan), w, plan, base=base).shape == (T, H)
+
+
+@pytest.mark.parametrize("part", ["order", "inverse", "offsets"])
+def test_a_plan_written_before_the_backward_pass_raises(plan, part):
+    for f in (lambda x: M.moe_dispatch(x, plan),
+              lambda x: M.moe_combine(x.repeat(K, 1), torch.ones(T, K), plan)):
+        x = torch.randn(T, H, requires_grad=True)
+        y = f(x)
+        getattr(plan, part).zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+
+
+def test_a_plan_of_the_callers_own_tensors(plan):
+    own = S.SortedTokens.__new__(S.SortedTokens)
+    own._mem, own._views = None, (plan.order.clone(), plan.inverse.clone(), plan.offsets.clone())
+    own._fill(*(t.data_ptr() for t in own._views), T, K, E, own._views[0].device)
+    x = torch.randn(T, H, requires_grad=True)
+    M.moe_dispatch(x, own).sum().backward()
+    assert torch.equal(x.grad, torch.full((T, H), float(K)))
+    y = M.moe_dispatch(x, own)
+    own._views[1].add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_a_plan_made_in_inference_mode(plan):
+    with torch.inference_mode():
+        p = S.SortedTokens._of(plan._mem.clone(), T, K, E)
+    x = torch.randn(T, H, requires_grad=True)
+    M.moe_combine(M.moe_dispatch(x, p), torch.ones(T, K), p).sum().backward()
+    assert torch.equal(x.grad, torch.full((T, H), float(K)))

@@ -15,6 +15,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/api/include/torch/version.h>
 
 #include <algorithm>
 #include <exception>
@@ -351,4 +352,11 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_minirun_torch", nullptr, -1, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__minirun_torch() { return PyModule_Create(&module_def); }
+PyMODINIT_FUNC PyInit__minirun_torch() {
+  PyObject* m = PyModule_Create(&module_def);
+  if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION)) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import warnings
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # MINIRUN_MOE_LIB selects another build of the same library (e.g. one built
@@ -251,23 +252,42 @@ TORCH_PATH = os.path.join(_HERE, "_lib", "_minirun_torch.so")
 _torch_ext = None
 
 
+class _NoShortWay:
+    """In the module's place where it was not built or does not load: takes no call."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def load_torch():
     """The module that takes torch tensors straight to the library (csrc/mr_torch.cpp), bound to
-    the loaded library. Raises LibraryMissing if it was not built."""
+    the loaded library. A build without it (``make lib``) has the same calls by ctypes, at twice
+    the host time; so has one made for another torch, which warns."""
     global _torch_ext
     if _torch_ext is None:
-        import importlib.machinery
-        import importlib.util
+        ext = _open_short_way() if os.path.exists(TORCH_PATH) else None
+        if ext is not None:
+            lib = load()
+            ext.bind(*(C.cast(getattr(lib, n), vp).value for n in _TORCH_API))
+        _torch_ext = ext or _NoShortWay()
+    return _torch_ext
 
-        import torch  # noqa: F401  (its libraries first)
-        if not os.path.exists(TORCH_PATH):
-            raise LibraryMissing(f"{TORCH_PATH} is missing: build it with "
-                                 "`make -C minirun-app_b200/csrc`")
-        loader = importlib.machinery.ExtensionFileLoader("_minirun_torch", TORCH_PATH)
+
+def _open_short_way():
+    import importlib.machinery
+    import importlib.util
+
+    import torch  # (its libraries first)
+    loader = importlib.machinery.ExtensionFileLoader("_minirun_torch", TORCH_PATH)
+    try:
         ext = importlib.util.module_from_spec(
             importlib.util.spec_from_loader("_minirun_torch", loader))
         loader.exec_module(ext)
-        lib = load()
-        ext.bind(*(C.cast(getattr(lib, n), vp).value for n in _TORCH_API))
-        _torch_ext = ext
-    return _torch_ext
+        if torch.__version__.startswith(ext.torch_version):
+            return ext
+        why = f"made for torch {ext.torch_version}, this is {torch.__version__}"
+    except ImportError as e:
+        why = str(e)
+    warnings.warn(f"{TORCH_PATH} is not used ({why}): calls go by ctypes; build it again with "
+                  "`make -C minirun-app_b200/csrc`", stacklevel=3)
+    return None

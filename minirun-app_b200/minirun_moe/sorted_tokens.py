@@ -70,7 +70,10 @@ class SortedTokens:
 
     def _split(self):
         if self._views is None:
-            self._views = L.load_torch().views(self._mem, self.tokens, self.top_k, self.experts)
+            P, E = self.rows, self.experts
+            self._views = L.load_torch().views(self._mem, self.tokens, self.top_k, E) or (
+                self._mem[:P], self._mem[P:2 * P].view(self.tokens, self.top_k),
+                self._mem[2 * P:2 * P + E + 1])
         return self._views
 
     def _version(self) -> tuple:

@@ -122,3 +122,27 @@ def test_a_values_flag_without_a_truth_value():
     x = torch.zeros((2, 64), device=dev())
     with pytest.raises(RuntimeError, match="ambiguous"):
         M.mxfp4_quantize(x, values=torch.zeros(2))
+
+
+def test_without_the_short_way_the_results_are_the_same(monkeypatch):
+    T, k, E, H, I = 40, 3, 6, 128, 64
+    ids = torch.from_numpy(choice(T, k, E, 1, 0.2)).to(dev())
+    x = torch.randn((T, H), generator=torch.Generator().manual_seed(2)).bfloat16().to(dev())
+    w = torch.rand((T, k), generator=torch.Generator().manual_seed(3)).to(dev())
+    stack = M.mxfp4_quantize(torch.randn((E, 2 * I, H), device=dev()))
+    one = M.MXFP4Weights(stack.packed[0], stack.scales[0])
+
+    def everything():
+        p = M.moe_sort(ids, E)
+        xs = M.moe_dispatch(x, p)
+        q, v = M.mxfp4_quantize(x, values=True)
+        mid = M.mxfp4_grouped_mm(q, stack, p, by_token=True)
+        h = M.mxfp4_quantize_swiglu(mid)
+        return (p.order, p.inverse, p.offsets, xs, M.moe_combine(xs, w, p),
+                M.moe_dispatch_backward(xs, p), *M.moe_combine_backward(x, xs, w, p), q.packed,
+                q.scales, v, mid, h.packed, h.scales, M.mxfp4_scaled_mm(q, one))
+
+    first = everything()
+    monkeypatch.setattr(L, "_torch_ext", L._NoShortWay())
+    for a, b in zip(first, everything(), strict=True):
+        assert torch.equal(a, b)

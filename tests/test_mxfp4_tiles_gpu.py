@@ -96,3 +96,39 @@ def test_clusters_end_together(counts, out, width, by_token):
     for _ in range(20):
         assert torch.equal(first, M.mxfp4_grouped_mm(a, w, p, by_token=by_token))
     assert bool((first[sum(counts):] == 0).all())
+
+
+def uneven(experts, mean, seed):
+    """Rows of each expert, from none to twice the mean."""
+    n = np.random.default_rng(seed).integers(0, 2 * mean + 1, experts)
+    n[seed % experts] = 0
+    return n.tolist()
+
+
+# Every CTA or pair of 148 SMs takes three tiles at least, so that both accumulators, the rings and
+# the exponents loaded ahead are used again, for tiles whose widths differ.
+PIPELINES = [  # experts, mean rows, weight rows, widths with aligned exponents and without
+    (128, 4, 648, (512, 1056)),    # tiles of 16 rows
+    (64, 8, 1160, (2048, 2080)),   # 32
+    (32, 18, 2568, (1024, 1056)),  # 64
+    (24, 36, 2600, (1024, 544)),   # 128, by pairs of CTAs
+    (8, 200, 4680, (512, 544)),    # 176
+]
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("by_token", [False, True])
+@pytest.mark.parametrize("experts,mean,out,widths", PIPELINES)
+def test_many_tiles_a_cta(experts, mean, out, widths, by_token, aligned):
+    width = widths[0 if aligned else 1]
+    counts = uneven(experts, mean, experts + mean)
+    check_grouped(counts, out, width, by_token, experts, dropped=experts // 4,
+                  out_dtype=torch.float32 if by_token == aligned else torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,out,width", [(1500, 9001, 512), (1500, 9001, 544),
+                                            (1061, 6200, 3104), (1061, 6200, 2560)])
+def test_many_tiles_of_one_matrix(rows, out, width):
+    a, w = matrix(rows, width, 1), matrix(out, width, 2)
+    A, W = values(a), values(w)
+    check(M.mxfp4_scaled_mm(a, w), A @ W.T, A.abs() @ W.abs().T, width)

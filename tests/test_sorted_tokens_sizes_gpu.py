@@ -146,3 +146,49 @@ def test_without_the_short_way_the_results_are_the_same(monkeypatch):
     monkeypatch.setattr(L, "_torch_ext", L._NoShortWay())
     for a, b in zip(first, everything(), strict=True):
         assert torch.equal(a, b)
+
+
+HALF_ULP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+def within(got, ref, mag, n, dtype):
+    """An fp32 sum of n products is within n * 2^-24 of their magnitudes' sum in any order; the
+    result's rounding adds half an ulp (and half an f16 subnormal step)."""
+    tol = (n + 2) * 2.0 ** -24 * mag + HALF_ULP[dtype] * (ref.abs() + mag * 2.0 ** -20)
+    over = (got.double() - ref).abs() - tol - (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert bool((over <= 0).all()), float(over.max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,k,H", [
+    (20011, 8, 96), (20011, 11, 96), (20011, 8, 131), (20011, 11, 131),  # eight slots a group
+    (6007, 8, 96), (401, 8, 2048), (401, 7, 2050),                       # four
+    (1501, 9, 2048), (801, 3, 520), (3001, 16, 260),                     # rows of several warps
+])
+def test_gradients_of_many_tokens(T, k, H, dtype):
+    """Batches that fill the GPU take several slots in one group of threads."""
+    ids = choice(T, k, 37, T + k, 0.1)
+    p = M.moe_sort(torch.from_numpy(ids).to(dev()), 37)
+    g = torch.Generator(device=dev()).manual_seed(H)
+    ys, dout = (torch.randn((n, H), generator=g, device=dev()).to(dtype) for n in (T * k, T))
+    w = torch.rand((T, k), generator=g, device=dev()) + 0.1
+    inv = torch.from_numpy(np_plan(ids, 37)[1]).to(dev()).long()
+    out, dx = M.moe_combine(ys, w, p), M.moe_dispatch_backward(ys, p)
+    dys, dw = M.moe_combine_backward(dout, ys, w, p)
+    ref, mag, rx, mx = (torch.zeros((T, H), dtype=torch.float64, device=dev()) for _ in range(4))
+    for j in range(k):  # one slot of all tokens after another
+        held = inv[:, j] >= 0
+        r = inv[held, j]
+        y, d, wj = ys[r].double(), dout[held].double(), w[held, j].double().unsqueeze(1)
+        ref[held] += wj * y
+        mag[held] += wj * y.abs()
+        rx[held] += y
+        mx[held] += y.abs()
+        within(dys[r], wj * d, (wj * d).abs(), 1, dtype)
+        within(dw[held, j], (d * y).sum(1), (d * y).abs().sum(1), H, torch.float32)
+        assert bool((dw[~held, j] == 0).all())
+    assert bool((dys[int(p.offsets[-1]):] == 0).all())
+    within(out, ref, mag, k, dtype)
+    within(dx, rx, mx, k, dtype)
+    again = M.moe_combine_backward(dout, ys, w, p)
+    assert torch.equal(dys, again[0]) and torch.equal(dw, again[1])

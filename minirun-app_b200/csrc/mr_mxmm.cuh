@@ -902,14 +902,15 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       }
       for (int c = 0; c < it.n; c += 16) {
         float v[16];
-        __syncwarp();  // the lanes' stores below may differ
+        __syncwarp();  // lanes without a weight row skip the stores below
         tmem_ld16(d_t + c, v);
-        const int left = o < p.out_features ? it.n - c : 0;
-        const int64_t at = ((int64_t)it.row0 + c) * p.out_features + o;
-        if (p.out_f32)
-          store16(reinterpret_cast<float*>(p.out) + at, p.out_features, left, v);
-        else
-          store16(reinterpret_cast<uint16_t*>(p.out) + at, p.out_features, left, v);
+        if (o < p.out_features) {
+          const int64_t at = ((int64_t)it.row0 + c) * p.out_features + o;
+          if (p.out_f32)
+            store16(reinterpret_cast<float*>(p.out) + at, p.out_features, it.n - c, v);
+          else
+            store16(reinterpret_cast<uint16_t*>(p.out) + at, p.out_features, it.n - c, v);
+        }
       }
       tc_fence_before();
       __syncwarp();

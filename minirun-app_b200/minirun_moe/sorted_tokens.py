@@ -278,22 +278,15 @@ class _Combine(torch.autograd.Function):
         return dys, dw, None, dout if ctx.needs_input_grad[3] else None
 
 
-def _recorded(*tensors) -> bool:
-    """Whether autograd has a part in the call: a gradient to record, or a tangent, which the
-    autograd functions refuse."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    if forward_ad._current_level >= 0:
-        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None
-                   for t in tensors)
-    return False
+def _dual(*tensors) -> bool:
+    """Whether one carries a forward-mode tangent (which the autograd functions refuse)."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def moe_dispatch(x: torch.Tensor, plan: SortedTokens) -> torch.Tensor:
     """``xs[r] = x[order[r] // top_k]`` [tokens * top_k, hidden]; rows without a pair are zero."""
-    if _recorded(x):
+    if (x.requires_grad and torch.is_grad_enabled()) or (
+            forward_ad._current_level >= 0 and _dual(x)):
         return _Dispatch.apply(x, plan)
     return _dispatch(x, plan)
 
@@ -302,6 +295,8 @@ def moe_combine(ys: torch.Tensor, weights: torch.Tensor, plan: SortedTokens,
                 base: torch.Tensor | None = None) -> torch.Tensor:
     """``out[t] = base[t] + sum_j weights[t, j] * ys[inverse[t, j]]``: fp32 sums in slot order,
     one rounding to the type of ``ys``. ``base``: rows to add (the shared expert's)."""
-    if _recorded(ys, weights, base):
+    if ((ys.requires_grad or weights.requires_grad or
+         (base is not None and base.requires_grad)) and torch.is_grad_enabled()) or (
+            forward_ad._current_level >= 0 and _dual(ys, weights, base)):
         return _Combine.apply(ys, weights, plan, base)
     return _combine(ys, weights, plan, base)

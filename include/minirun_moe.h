@@ -267,7 +267,8 @@ typedef struct mr_sorted {
 /* ids int32 [tokens, top_k] -> order, inverse, offsets (device buffers). An id
  * of -1 is a slot without an expert (one held by another rank, a dropped
  * token); any other id outside [0, experts) is treated so too and sets
- * MR_DEVERR_BAD_EXPERT_ID. Deterministic. */
+ * MR_DEVERR_BAD_EXPERT_ID. Deterministic. More than 4096 pairs are sorted by
+ * a cluster of 16 CTAs: a part of a GPU that cannot place one gives MR_ERR_CUDA. */
 mr_status mr_moe_sort(mr_ctx* ctx, const int32_t* ids, int64_t tokens, int32_t top_k,
                       int32_t experts, int32_t* order, int32_t* inverse, int32_t* offsets,
                       void* stream);

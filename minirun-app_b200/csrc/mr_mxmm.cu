@@ -92,8 +92,8 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
   // Tile width: three times an expert's mean rows, so that few experts need a
   // second tile, which would load their weights again; narrow tiles leave room
   // for a deeper ring. Against twice the mean, 256 experts of 1024 x 3584 and
-  // 8 slots a token: 512 tokens 83 -> 81 us and 1024 83 -> 86 with even experts,
-  // 91 -> 83 and 97 -> 90 where the most popular has ten times the mean; four
+  // 8 slots a token: 512 tokens 84 -> 82 us and 1024 84 -> 86 with even experts,
+  // 91 -> 83 and 100 -> 90 where the most popular has ten times the mean; four
   // times is as good as three. Tiles are at most one per expert with rows and
   // the full ones.
   const int64_t mean = plan ? (rows + p.E - 1) / p.E : rows;
@@ -110,7 +110,7 @@ mr_status product(mr_ctx* ctx, const mr_mxfp4_desc* a, const mr_mxfp4_desc* w,
     return fail(ctx, MR_ERR_UNSUPPORTED, "the product has more than 2^31 tiles");
   p.ksplit = 1;
   // CTAs share a tile where there are few, the rows are long and the tile is
-  // narrow (1 and 16 rows x 2048 x 7168 in L2: 8.2 -> 6.2 us and 8.1 -> 6.8; with 32
+  // narrow (1 and 16 rows x 2048 x 7168 in L2: 8.3 -> 6.5 us and 8.1 -> 6.8; with 32
   // rows, or rows of 2048, the exchange costs what the shorter loop saves).
   while (p.ntile == 16 && p.ksplit < kMmSplit && 2 * p.ksplit * tiles <= sms && p.nstages >= 8)
     p.ksplit *= 2;

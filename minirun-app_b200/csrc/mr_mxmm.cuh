@@ -12,16 +12,22 @@
 // CG = 1: one CTA a tile. CG = 2: a cluster of two CTAs a tile of 256 weight
 // rows; each loads its own 128 rows and half of the activations, and the
 // leader's MMAs (cta_group::2) read both halves: per stage of 176 rows a CTA
-// takes 54 KB of codes from L2 instead of 76. That is what bounds a large
-// product: an SM takes 64 bytes a cycle from L2, so a stage of n rows is
-// 512 + 2n cycles of loads (512 + 4n without the pair) against 4n of MMAs.
+// takes 54 KB of codes from L2 instead of 76. At 64 bytes a cycle from L2 to an
+// SM a stage of n rows is 512 + 2n cycles of loads (512 + 4n without the pair)
+// against 4n of MMAs.
 //
-// Measured, out bf16: 4096 x 16384 x 7168 209 us (4.6 PFLOP/s); 64 tokens x 8
-// of 256 experts of 2048 x 7168 256 us (0.99 of the copy rate, the weights);
-// one token x 8 of them 14.7 us (floor 9.5): the first copy starts 2.8 us after
+// Measured, out bf16: 4096 x 16384 x 7168 200 to 209 us (4.6 to 4.8 PFLOP/s; 230
+// in a loop of two seconds, at 1.2 GHz under the power cap); 64 tokens x 8 of 256
+// experts of 2048 x 7168 252 us (the weights at 6.9 TB/s). 2048 tokens x 8 of 32
+// experts 118 us sorted and 134 by token, tiles of 148 rows: a stage takes 0.70
+// and 0.80 us, 1110 and 1470 cycles at the clocks of a loop of two seconds, where
+// the loads need 808 and the MMAs 592. Neither is the bound (1024 tokens: tensor
+// pipe active 41 % of the time, L2 38 %); most likely the three or four slots of
+// the ring do not cover the loads' latency, 1200-1900 cycles.
+// One token x 8 of 256 14.3 us (floor 9.5): the first copy starts 2.8 us after
 // the kernel does (the table 1.3, the rest the fetch of each role's code), the
 // last tile's result leaves 1.1 us after its codes are there, and between the
-// two HBM runs at 0.99. One row x 2048 x 7168 7.4 us, 6.3 with the weights in
+// two HBM runs at 0.99. One row x 2048 x 7168 7.4 us, 6.5 with the weights in
 // L2. (Tried for the start, each within 1 % or slower: the first weights'
 // copies right behind the table, 10.2 -> 11.1 us at 64 experts of 1024 x 4096;
 // the table's code run once on nothing before the wait for the kernels ahead;
@@ -272,7 +278,10 @@ MR_DEVICE void arrive_all(uint64_t* bar, int ctas) {
 // The last thing a thread of a cluster of CTAs does: what it did to another
 // CTA's memory is done, and it waits for all threads of the cluster that have
 // not ended to say the same. (The CTAs' own barriers cannot serve for this: a
-// CTA whose wait expired leaves its further waits early.)
+// CTA whose wait expired leaves its further waits early.) At least one lane of
+// every warp has to come here: with whole warps gone for good the barrier does
+// not complete. It costs a pair of CTAs 0.3 to 0.6 us of a call (77 x 2048 x
+// 7168), a split tile's CTAs nothing.
 MR_DEVICE void leave_cluster() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");

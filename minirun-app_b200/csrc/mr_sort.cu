@@ -65,7 +65,9 @@ MR_DEVICE unsigned lanes_with(unsigned key, int bits) {
 // the histograms into first rows, pass 2 hands out the rows. The grid is one
 // cluster (or one CTA); blockDim.x >= E. Latency-bound: ids, then the
 // cluster barrier, then the scattered rows. 256 experts: 32 pairs 2 us, 32768
-// 7.2 us (one CTA 13.7), 65536 9 us (22).
+// 7.6 us (one CTA 13.7), 65536 9 us (22). More than 4096 pairs need a GPU (or a
+// part of one) that places 16 CTAs of one cluster; where it cannot, the launch
+// fails and the call says so.
 __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) {
   extern __shared__ int hist[];  // [warps][E], then [E] CTA totals, [E] first rows, [32]
   cg::cluster_group cluster = cg::this_cluster();

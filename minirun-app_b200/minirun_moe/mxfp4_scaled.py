@@ -52,7 +52,8 @@ def _weights_of(packed: torch.Tensor, scales: torch.Tensor, rows: int, width: in
 def mxfp4_quantize(x: torch.Tensor, values: bool = False):
     """``x`` [rows, in] or [experts, rows, in] in MXFP4 (see mr_mxfp4_quantize for the rounding).
     With ``values`` the pair (codes, values): the numbers the codes stand for in x's type, what a
-    training step with 4-bit forward values multiplies with."""
+    training step with 4-bit forward values multiplies with. No gradient is recorded: how it passes
+    the rounding is the caller's choice (straight through: ``x + (values - x.detach())``)."""
     if x.is_cuda and x.dim() == 2:
         ctx = Context.get(x.get_device())
         r = L.load_torch().quantize(ctx.address, ctx.device, x, values)

@@ -279,8 +279,9 @@ MR_DEVICE void arrive_all(uint64_t* bar, int ctas) {
 // CTA's memory is done, and it waits for all threads of the cluster that have
 // not ended to say the same. (The CTAs' own barriers cannot serve for this: a
 // CTA whose wait expired leaves its further waits early.) At least one lane of
-// every warp has to come here: with whole warps gone for good the barrier does
-// not complete. It costs a pair of CTAs 0.3 to 0.6 us of a call (77 x 2048 x
+// every warp has to come here, and the lanes that do together (__syncwarp in
+// the roles of whole warps): with whole warps gone for good the barrier did not
+// complete. It costs a pair of CTAs 0.3 to 0.6 us of a call (77 x 2048 x
 // 7168), a split tile's CTAs nothing.
 MR_DEVICE void leave_cluster() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -752,6 +753,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
     else
       mm_load_scales<mm_max_b(CG), WIDE, false>(p, it, lane, first, stride, n_items, st0, st1,
                                                        raw, rfull, rempty, flags);
+    __syncwarp();
   } else if (warp >= 8 && warp < 12) {
     // -------------------------------------------- exponents to tensor memory
     const uint32_t lane_t = tbase + ((uint32_t)((warp & 3) * 32) << 16) + 2 * p.ntile;
@@ -806,6 +808,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
         }
       }
     if (lane == 0) mbar_arrive(done);
+    __syncwarp();
   } else if (warp >= 12) {
     // -------------------------------------------------------------- gathers
     if (!elect_one()) return;
@@ -951,6 +954,7 @@ __global__ void __launch_bounds__(kMmThreads + 32 * kMmGatherWarps, 1)
       else
         reinterpret_cast<uint16_t*>(p.out)[i] = 0;
     }
+    __syncwarp();
   }
   if (CG * ks > 1) leave_cluster();
 }

@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
     }
     // no CTA leaves (below) before the others have read its totals; not the
     // .aligned forms: a warp's lanes may have parted above
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   }
   // exclusive scan over the experts
@@ -188,7 +189,10 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortParams p) 
   for (int64_t r = kept + (int64_t)rank * blockDim.x + tid; r < p.P;
        r += (int64_t)ctas * blockDim.x)
     p.order[r] = -1;
-  if (ctas > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  if (ctas > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  }
 }
 
 // ------------------------------------------------------------- row copies

@@ -281,7 +281,8 @@ MR_DEVICE void arrive_all(uint64_t* bar, int ctas) {
 // CTA whose wait expired leaves its further waits early.) At least one lane of
 // every warp has to come here, and the lanes that do together (__syncwarp in
 // the roles of whole warps): with whole warps gone for good the barrier did not
-// complete. It costs a pair of CTAs 0.3 to 0.6 us of a call (77 x 2048 x
+// complete. It has no limit of its own: every wait before it is bounded, so all
+// come here. It costs a pair of CTAs 0.3 to 0.6 us of a call (77 x 2048 x
 // 7168), a split tile's CTAs nothing.
 MR_DEVICE void leave_cluster() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
